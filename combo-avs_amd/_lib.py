@@ -132,13 +132,19 @@ _SIGNATURES = {
     "combo_attention_backward_f32": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p] + [c_int] * 5 + [c_float] + [c_void_p] * 8,
     "combo_attention_backward_ld_f32": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p] + [c_int] * 5 + [c_float]
                                        + [c_void_p] * 6 + [c_longlong, c_void_p, c_longlong, c_void_p],
+    "combo_groupnorm_act_workspace": [c_int] * 6,
+    "combo_groupnorm_act_forward": [c_void_p] * 3 + [c_int] * 4 + [c_float, c_int, c_int] + [c_void_p] * 5,
+    "combo_groupnorm_act_backward": [c_void_p] * 6 + [c_int] * 6 + [c_void_p] * 5,
+    "combo_rotary_axes": [c_void_p] + [c_longlong] * 3 + [c_int, c_void_p, c_int] + [c_longlong] * 3 + [c_int] * 5 + [c_void_p, c_void_p, c_int, c_int,
+                          c_void_p, c_void_p],
     "combo_adamw_f32": [c_void_p] * 4 + [c_longlong, c_void_p] + [c_float] * 7 + [c_void_p],
     "combo_sra_attention_ok": [c_int, c_int, c_int],
     "combo_sra_attention_backward_workspace": [c_int, c_int, c_int, c_int],
     "combo_sra_attention_forward_bf16": [c_void_p] * 4 + [c_int] * 4 + [c_float, c_void_p],
     "combo_sra_attention_backward_bf16": [c_void_p] * 9 + [c_int] * 4 + [c_float, c_void_p],
 }
-_RESTYPES = {"combo_build_arch": ctypes.c_char_p, "combo_sra_attention_backward_workspace": ctypes.c_longlong}
+_RESTYPES = {"combo_build_arch": ctypes.c_char_p, "combo_sra_attention_backward_workspace": ctypes.c_longlong,
+             "combo_groupnorm_act_workspace": ctypes.c_longlong}
 
 
 def exported_symbols():
@@ -172,6 +178,14 @@ def check(code, what):
         raise HipError(f"{what} failed with hipError_t {code}")
 
 
+def _float_types():
+    import torch
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+FLOAT_TYPES = _float_types()  # dtype codes of the entry points that take several types
+
+
 def ptr(t):
     """Device pointer of a contiguous torch tensor (None -> NULL)."""
     return 0 if t is None else t.data_ptr()
@@ -180,6 +194,26 @@ def ptr(t):
 def current_stream():
     import torch
     return torch.cuda.current_stream().cuda_stream
+
+
+
+
+class device_of:
+    """`with device_of(t) as stream:` t's device is current inside the block; stream: that device's current stream"""
+
+    def __init__(self, t):
+        self.index, self.guard = t.device.index, None
+
+    def __enter__(self):
+        import torch
+        if self.index is not None and self.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+        return current_stream()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def require_cuda(*tensors, channels_last=False):

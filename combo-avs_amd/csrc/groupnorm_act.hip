@@ -1,0 +1,600 @@
+// Group norm with an activation on channels-last maps [B, HW, C] of fp32, bf16 or fp16, any channel count, forward and backward:
+//     z = (x - mean[b, g]) rstd[b, g] w[c] + bias[c],  y = act(z),  act = none, ReLU, SiLU or GELU (erf)
+//     dz = dy act'(z);  db[c] = sum dz;  dw[c] = sum dz xh;  dx = rstd (dz w - mean_g(dz w) - xh mean_g(dz w xh)),  xh = (x - mean) rstd
+// The backward pass recomputes z from x: nothing but mean and rstd is kept, and the activation costs no tensor of its own.
+//
+// Bound: HBM.  A thread owns V neighbouring channels (16 bytes where the channel count and the pointers allow it) and walks the tokens, so
+// per-channel constants stay in registers and all accesses are whole vectors.  Two shapes:
+//   one launch   a workgroup owns one image and a few whole groups: it reads them for the statistics and again, out of the cache, for the
+//                result.  For maps whose slice per workgroup is small (the launch then costs more than the traffic).
+//   two launches partial statistics per (image, slice of tokens), then every workgroup of the second launch joins the partials of its own
+//                image - a few KB out of L2 - and writes its tokens.
+// Statistics: a thread sums x - K and (x - K)^2 with K its own first value of the channel, in fp32, and hands on (mean, M2); these are
+// joined as M2 = sum M2_i + sum n_i (mean_i - mean)^2.  K is one of the values, so the shift's cancellation is at most n_thread * 2^-24 of M2
+// whatever the offset of the map (a plain sum of squares loses everything once mean^2 > 2^24 var).  All sums have a fixed order.
+#include "combo_common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxC = 4096;  // (a token's channel statistics and group results lie in 64 KiB of LDS)
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec { T v[V]; };
+
+template <int ACT>
+__device__ __forceinline__ float act(float z) {
+  if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;  // (a NaN stays one)
+  if constexpr (ACT == ACT_SILU) return z / (1.f + __expf(-z));
+  if constexpr (ACT == ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  return z;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if constexpr (ACT == ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if constexpr (ACT == ACT_SILU) {
+    const float s = 1.f / (1.f + __expf(-z));
+    return s * (1.f + z * (1.f - s));
+  }
+  if constexpr (ACT == ACT_GELU) return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+  return 1.f;
+}
+
+struct NormArgs {
+  const void *x, *dy;
+  const float *w, *bias;      // nullable
+  float *mean, *rstd;         // [B][G]
+  float *part;                // forward: [B][S][G][2] (mean, M2); backward: [B][S][G][2] (s1, s2), then [B * S][C][2] (u, v)
+  float *dw, *db;             // nullable
+  void* out;
+  float eps;
+  int B, HW, C, G, per, S, slice;  // per: channels of a group; slice: tokens of a partial
+  int range;                       // channels of a workgroup (the one-launch shape; else C)
+};
+
+// How a workgroup lies over [tokens][channels c0 .. c0 + range): a row of `width` threads covers the vectors of a token, `rows` such rows
+// walk the tokens; a range of more than 256 vectors is walked in several sets.
+struct Lanes {
+  int width, rows, row, chunk;
+  bool on;
+  __device__ Lanes(int vectors) {
+    width = min(vectors, kThreads);
+    rows = kThreads / width;
+    row = threadIdx.x / width;
+    chunk = threadIdx.x - row * width;
+    on = row < rows;
+  }
+};
+
+__device__ __forceinline__ float team_sum(float v, int team) {
+  for (int o = team >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// threads of a team that joins one group: a power of two <= 64 so that a team lies inside a wave
+__device__ __forceinline__ int team_size(int groups) {
+  int t = 64;
+  while (t > 1 && kThreads / t < groups) t >>= 1;
+  return t;
+}
+
+// (mean, M2) of `entries` (mean_i, M2_i, n_i): get(i, n, m, M2)
+template <typename F>
+__device__ __forceinline__ void join_stats(int entries, int team, int lane, F get, float& n, float& mean, float& M2) {
+  float sn = 0.f, sm = 0.f;
+  for (int i = lane; i < entries; i += team) {
+    float ni, mi, qi;
+    get(i, ni, mi, qi);
+    sn += ni;
+    sm += ni * mi;
+  }
+  n = team_sum(sn, team);
+  mean = n > 0.f ? team_sum(sm, team) / n : 0.f;
+  float q = 0.f;
+  for (int i = lane; i < entries; i += team) {
+    float ni, mi, qi;
+    get(i, ni, mi, qi);
+    if (ni > 0.f) q += qi + ni * (mi - mean) * (mi - mean);
+  }
+  M2 = team_sum(q, team);
+}
+
+// per-channel (mean, M2) of a token range into LDS: stat[rows][range][2]
+template <typename T, int V>
+__device__ __forceinline__ void channel_stats(const T* x, int C, int range, int t0, int t1, const Lanes& L, float* stat) {
+  if (!L.on) return;
+  for (int ch = L.chunk; ch * V < range; ch += kThreads) {
+    const T* p = x + (long long)(t0 + L.row) * C + ch * V;
+    float K[V], s[V], q[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) K[k] = s[k] = q[k] = 0.f;
+    int n = 0;
+    if (t0 + L.row < t1) {
+      const Vec<T, V> a = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+      for (int k = 0; k < V; ++k) K[k] = (float)a.v[k];
+      n = (t1 - t0 - L.row + L.rows - 1) / L.rows;
+      const long long step = (long long)L.rows * C;
+#pragma unroll 4
+      for (int i = 1; i < n; ++i) {
+        p += step;
+        const Vec<T, V> b = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float d = (float)b.v[k] - K[k];
+          s[k] += d;
+          q[k] += d * d;
+        }
+      }
+    }
+    const float inv = n > 0 ? 1.f / (float)n : 0.f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      float* o = stat + (L.row * range + ch * V + k) * 2;
+      o[0] = K[k] + s[k] * inv;
+      o[1] = q[k] - s[k] * s[k] * inv;
+    }
+  }
+}
+
+__device__ __forceinline__ void group_of_stat(const float* stat, int range, int per, int rows, int tokens, int g, int team, int lane, float& n,
+                                              float& mean, float& M2) {
+  join_stats(rows * per, team, lane,
+             [&](int i, float& ni, float& mi, float& qi) {
+               const int r = i / per, c = g * per + (i - r * per);
+               ni = r < tokens ? (float)((tokens - r + rows - 1) / rows) : 0.f;
+               mi = stat[(r * range + c) * 2];
+               qi = stat[(r * range + c) * 2 + 1];
+             },
+             n, mean, M2);
+}
+
+// partial statistics of one slice
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) gna_stats_kernel(const NormArgs A) {
+  extern __shared__ float sh[];
+  const int b = blockIdx.x / A.S, s = blockIdx.x - b * A.S;
+  const int t0 = s * A.slice, t1 = min(A.HW, t0 + A.slice);
+  const Lanes L(A.C / V);
+  channel_stats<T, V>(static_cast<const T*>(A.x) + (long long)b * A.HW * A.C, A.C, A.C, t0, t1, L, sh);
+  __syncthreads();
+  const int team = team_size(A.G), lane = threadIdx.x & (team - 1);
+  for (int g0 = 0; g0 < A.G; g0 += kThreads / team) {
+    const int g = g0 + threadIdx.x / team;
+    float n, mean, M2;
+    group_of_stat(sh, A.C, A.per, L.rows, t1 - t0, min(g, A.G - 1), team, lane, n, mean, M2);
+    if (lane == 0 && g < A.G) {
+      float* o = A.part + (((long long)b * A.S + s) * A.G + g) * 2;
+      o[0] = mean;
+      o[1] = M2;
+    }
+  }
+}
+
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void apply_tokens(const NormArgs& A, int b, int c0, int range, int t0, int t1, const Lanes& L, const float* mean,
+                                             const float* rstd) {
+  if (!L.on) return;
+  const T* x = static_cast<const T*>(A.x) + (long long)b * A.HW * A.C + c0;
+  T* y = static_cast<T*>(A.out) + (long long)b * A.HW * A.C + c0;
+  for (int ch = L.chunk; ch * V < range; ch += kThreads) {
+    float m[V], a[V], bb[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int c = ch * V + k, g = c / A.per;
+      m[k] = mean[g];
+      a[k] = rstd[g] * (A.w ? A.w[c0 + c] : 1.f);
+      bb[k] = A.bias ? A.bias[c0 + c] : 0.f;
+    }
+    long long off = (long long)(t0 + L.row) * A.C + ch * V;
+    const long long step = (long long)L.rows * A.C;
+#pragma unroll 4
+    for (int t = t0 + L.row; t < t1; t += L.rows, off += step) {
+      const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + off);
+      Vec<T, V> o;
+#pragma unroll
+      for (int k = 0; k < V; ++k) o.v[k] = (T)act<ACT>(((float)v.v[k] - m[k]) * a[k] + bb[k]);
+      *reinterpret_cast<Vec<T, V>*>(y + off) = o;
+    }
+  }
+}
+
+__device__ __forceinline__ float rstd_of(float M2, float n, float eps) { return 1.f / sqrtf(M2 / n + eps); }
+
+// second launch: joins the partials of its image, normalises its slice
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) gna_apply_kernel(const NormArgs A, int slice, int slices) {
+  extern __shared__ float sh[];  // mean[G], rstd[G]
+  const int b = blockIdx.x / slices, s = blockIdx.x - b * slices;
+  const int team = team_size(A.G), lane = threadIdx.x & (team - 1);
+  for (int g0 = 0; g0 < A.G; g0 += kThreads / team) {
+    const int g = min(g0 + (int)threadIdx.x / team, A.G - 1);
+    const float* part = A.part + ((long long)b * A.S * A.G + g) * 2;
+    float n, mean, M2;
+    join_stats(A.S, team, lane,
+               [&](int i, float& ni, float& mi, float& qi) {
+                 ni = (float)min(A.slice, A.HW - i * A.slice) * A.per;
+                 mi = part[(long long)i * A.G * 2];
+                 qi = part[(long long)i * A.G * 2 + 1];
+               },
+               n, mean, M2);
+    if (lane == 0) {
+      const float r = rstd_of(M2, n, A.eps);
+      sh[g] = mean;
+      sh[A.G + g] = r;
+      if (s == 0) {
+        A.mean[b * A.G + g] = mean;
+        A.rstd[b * A.G + g] = r;
+      }
+    }
+  }
+  __syncthreads();
+  const Lanes L(A.C / V);
+  apply_tokens<T, V, ACT>(A, b, 0, A.C, s * slice, min(A.HW, (s + 1) * slice), L, sh, sh + A.G);
+}
+
+// one launch: an image's channels [c0, c0 + range) by one workgroup
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) gna_forward_kernel(const NormArgs A) {
+  extern __shared__ float sh[];
+  const int parts = A.C / A.range, b = blockIdx.x / parts, c0 = (blockIdx.x - b * parts) * A.range;
+  const int gn = A.range / A.per, g00 = c0 / A.per;
+  const Lanes L(A.range / V);
+  channel_stats<T, V>(static_cast<const T*>(A.x) + (long long)b * A.HW * A.C + c0, A.C, A.range, 0, A.HW, L, sh);
+  __syncthreads();
+  float* mr = sh + (size_t)L.rows * A.range * 2;
+  const int team = team_size(gn), lane = threadIdx.x & (team - 1);
+  for (int g0 = 0; g0 < gn; g0 += kThreads / team) {
+    const int g = min(g0 + (int)threadIdx.x / team, gn - 1);
+    float n, mean, M2;
+    group_of_stat(sh, A.range, A.per, L.rows, A.HW, g, team, lane, n, mean, M2);
+    if (lane == 0) {
+      const float r = rstd_of(M2, n, A.eps);
+      mr[g] = mean;
+      mr[gn + g] = r;
+      A.mean[b * A.G + g00 + g] = mean;
+      A.rstd[b * A.G + g00 + g] = r;
+    }
+  }
+  __syncthreads();
+  apply_tokens<T, V, ACT>(A, b, c0, A.range, 0, A.HW, L, mr, mr + gn);
+}
+
+// ---- backward ----
+
+// per-channel (u, v) = (sum dz, sum dz xh) of a token range into LDS: uv[rows][range][2]
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void channel_grads(const NormArgs& A, int b, int c0, int range, int t0, int t1, const Lanes& L, float* uv) {
+  if (!L.on) return;
+  const T* x = static_cast<const T*>(A.x) + (long long)b * A.HW * A.C + c0;
+  const T* dy = static_cast<const T*>(A.dy) + (long long)b * A.HW * A.C + c0;
+  for (int ch = L.chunk; ch * V < range; ch += kThreads) {
+    float m[V], r[V], w[V], bb[V], u[V], v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int c = ch * V + k, g = b * A.G + (c0 + c) / A.per;
+      m[k] = A.mean[g];
+      r[k] = A.rstd[g];
+      w[k] = A.w ? A.w[c0 + c] : 1.f;
+      bb[k] = A.bias ? A.bias[c0 + c] : 0.f;
+      u[k] = v[k] = 0.f;
+    }
+    long long off = (long long)(t0 + L.row) * A.C + ch * V;
+    const long long step = (long long)L.rows * A.C;
+#pragma unroll 2
+    for (int t = t0 + L.row; t < t1; t += L.rows, off += step) {
+      const Vec<T, V> xv = *reinterpret_cast<const Vec<T, V>*>(x + off), gv = *reinterpret_cast<const Vec<T, V>*>(dy + off);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float xh = ((float)xv.v[k] - m[k]) * r[k];
+        const float dz = (float)gv.v[k] * act_slope<ACT>(xh * w[k] + bb[k]);
+        u[k] += dz;
+        v[k] += dz * xh;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      float* o = uv + (L.row * range + ch * V + k) * 2;
+      o[0] = u[k];
+      o[1] = v[k];
+    }
+  }
+}
+
+// joins the rows of uv[rows][range][2] into row 0, writes them to `chan` [range][2] and the group sums (sum_c w u, sum_c w v) to s12[gn][2]
+__device__ __forceinline__ void join_grads(const NormArgs& A, int c0, int range, const Lanes& L, float* uv, float* chan, float* s12) {
+  for (int i = threadIdx.x; i < range; i += kThreads) {
+    float u = 0.f, v = 0.f;
+    for (int r = 0; r < L.rows; ++r) {
+      u += uv[(r * range + i) * 2];
+      v += uv[(r * range + i) * 2 + 1];
+    }
+    chan[2 * i] = u;
+    chan[2 * i + 1] = v;
+    const float w = A.w ? A.w[c0 + i] : 1.f;
+    uv[2 * i] = u * w;
+    uv[2 * i + 1] = v * w;
+  }
+  __syncthreads();
+  const int gn = range / A.per, team = team_size(gn), lane = threadIdx.x & (team - 1);
+  for (int g0 = 0; g0 < gn; g0 += kThreads / team) {
+    const int g = min(g0 + (int)threadIdx.x / team, gn - 1);
+    float a = 0.f, q = 0.f;
+    for (int c = lane; c < A.per; c += team) {
+      a += uv[(g * A.per + c) * 2];
+      q += uv[(g * A.per + c) * 2 + 1];
+    }
+    a = team_sum(a, team);
+    q = team_sum(q, team);
+    if (lane == 0) {
+      s12[2 * g] = a;
+      s12[2 * g + 1] = q;
+    }
+  }
+}
+
+// s12: [gn][2] of this image's groups from c0 on
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void dx_tokens(const NormArgs& A, int b, int c0, int range, int t0, int t1, const Lanes& L, const float* s12) {
+  if (!L.on) return;
+  const long long base = (long long)b * A.HW * A.C + c0;
+  const T* x = static_cast<const T*>(A.x) + base;
+  const T* dy = static_cast<const T*>(A.dy) + base;
+  T* dx = static_cast<T*>(A.out) + base;
+  const float inv_n = 1.f / ((float)A.HW * (float)A.per);
+  for (int ch = L.chunk; ch * V < range; ch += kThreads) {
+    float m[V], r[V], w[V], bb[V], a1[V], a2[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int c = ch * V + k, gl = c / A.per, g = b * A.G + c0 / A.per + gl;
+      m[k] = A.mean[g];
+      r[k] = A.rstd[g];
+      w[k] = A.w ? A.w[c0 + c] : 1.f;
+      bb[k] = A.bias ? A.bias[c0 + c] : 0.f;
+      a1[k] = s12[2 * gl] * inv_n;
+      a2[k] = s12[2 * gl + 1] * inv_n;
+    }
+    long long off = (long long)(t0 + L.row) * A.C + ch * V;
+    const long long step = (long long)L.rows * A.C;
+#pragma unroll 2
+    for (int t = t0 + L.row; t < t1; t += L.rows, off += step) {
+      const Vec<T, V> xv = *reinterpret_cast<const Vec<T, V>*>(x + off), gv = *reinterpret_cast<const Vec<T, V>*>(dy + off);
+      Vec<T, V> o;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float xh = ((float)xv.v[k] - m[k]) * r[k];
+        const float dz = (float)gv.v[k] * act_slope<ACT>(xh * w[k] + bb[k]);
+        o.v[k] = (T)(r[k] * (dz * w[k] - a1[k] - xh * a2[k]));
+      }
+      *reinterpret_cast<Vec<T, V>*>(dx + off) = o;
+    }
+  }
+}
+
+__device__ __forceinline__ float* chan_of(const NormArgs& A) { return A.part + (long long)A.B * A.S * A.G * 2; }
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) gna_grad_partial_kernel(const NormArgs A) {
+  extern __shared__ float sh[];
+  const int b = blockIdx.x / A.S, s = blockIdx.x - b * A.S;
+  const Lanes L(A.C / V);
+  channel_grads<T, V, ACT>(A, b, 0, A.C, s * A.slice, min(A.HW, (s + 1) * A.slice), L, sh);
+  __syncthreads();
+  join_grads(A, 0, A.C, L, sh, chan_of(A) + (long long)blockIdx.x * A.C * 2, A.part + (long long)blockIdx.x * A.G * 2);
+}
+
+// dw, db: 16 channels by 16 rows of partials per workgroup, joined in a fixed order
+__device__ __forceinline__ void param_grads(const NormArgs& A, int block, int rows_total, float* sh) {
+  const int c = block * 16 + (threadIdx.x & 15), r0 = threadIdx.x >> 4;
+  const float* p = chan_of(A);
+  float u = 0.f, v = 0.f;
+  if (c < A.C) {
+#pragma unroll 4
+    for (int r = r0; r < rows_total; r += 16) {
+      const float2 a = *reinterpret_cast<const float2*>(p + ((long long)r * A.C + c) * 2);
+      u += a.x;
+      v += a.y;
+    }
+  }
+  sh[threadIdx.x] = u;
+  sh[256 + threadIdx.x] = v;
+  __syncthreads();
+  if (threadIdx.x < 16 && c < A.C) {
+    for (int r = 1; r < 16; ++r) {
+      u += sh[r * 16 + threadIdx.x];
+      v += sh[256 + r * 16 + threadIdx.x];
+    }
+    if (A.dw) A.dw[c] = v;
+    if (A.db) A.db[c] = u;
+  }
+}
+
+// second launch: the first workgroups join dw and db, the others write dx
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) gna_grad_apply_kernel(const NormArgs A, int slice, int slices, int param_blocks) {
+  extern __shared__ float sh[];
+  if ((int)blockIdx.x < param_blocks) {
+    param_grads(A, blockIdx.x, A.B * A.S, sh);
+    return;
+  }
+  const int id = blockIdx.x - param_blocks, b = id / slices, s = id - b * slices;
+  const int team = team_size(A.G), lane = threadIdx.x & (team - 1);
+  for (int g0 = 0; g0 < A.G; g0 += kThreads / team) {
+    const int g = min(g0 + (int)threadIdx.x / team, A.G - 1);
+    float a = 0.f, q = 0.f;
+    for (int i = lane; i < A.S; i += team) {
+      const float* p = A.part + (((long long)b * A.S + i) * A.G + g) * 2;
+      a += p[0];
+      q += p[1];
+    }
+    a = team_sum(a, team);
+    q = team_sum(q, team);
+    if (lane == 0) {
+      sh[2 * g] = a;
+      sh[2 * g + 1] = q;
+    }
+  }
+  __syncthreads();
+  const Lanes L(A.C / V);
+  dx_tokens<T, V, ACT>(A, b, 0, A.C, s * slice, min(A.HW, (s + 1) * slice), L, sh);
+}
+
+// one launch for dx (S = 1: the channel sums of an image are one row of partials); dw and db follow in gna_param_kernel
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) gna_backward_kernel(const NormArgs A) {
+  extern __shared__ float sh[];
+  const int parts = A.C / A.range, b = blockIdx.x / parts, c0 = (blockIdx.x - b * parts) * A.range;
+  const Lanes L(A.range / V);
+  float* s12 = sh + (size_t)L.rows * A.range * 2;
+  channel_grads<T, V, ACT>(A, b, c0, A.range, 0, A.HW, L, sh);
+  __syncthreads();
+  join_grads(A, c0, A.range, L, sh, chan_of(A) + ((long long)b * A.C + c0) * 2, s12);
+  __syncthreads();
+  dx_tokens<T, V, ACT>(A, b, c0, A.range, 0, A.HW, L, s12);
+}
+
+__global__ void __launch_bounds__(kThreads) gna_param_kernel(const NormArgs A) {
+  __shared__ float sh[512];
+  param_grads(A, blockIdx.x, A.B, sh);
+}
+
+// ---- host ----
+
+// channels of a workgroup in the one-launch shape: the fewest whole groups that make whole vectors and at least a cache line
+int channel_range(int C, int G, int V, int size) {
+  const int per = C / G;
+  for (int k = 1; k < G; ++k)
+    if (G % k == 0 && (k * per) % V == 0 && k * per * size >= 128) return k * per;
+  return C;
+}
+
+int vector_of(int C, int size, uintptr_t all) {
+  int V = 16 / size;
+  while (V > 1 && (C % V || all % (V * size))) V >>= 1;
+  return V;
+}
+
+// One launch while a workgroup's slice is at most 128 KiB, i.e. at most ~4 us of one CU's cache traffic, less than a second launch and
+// its join cost; a large map goes over the whole chip in two.
+bool one_launch(const NormArgs& A, int size) { return (long long)A.HW * A.range * size <= 131072; }
+
+size_t lds_floats(int range, int V) {
+  const int vectors = range / V, rows = vectors < kThreads ? kThreads / vectors : 1;
+  return (size_t)rows * range * 2;
+}
+
+// slices of an image: >= 1024 workgroups over the batch where the map is large, at least 16 tokens and 16 KiB in each
+void choose_slices(NormArgs& A, int size) {
+  long long by_bytes = ((long long)A.HW * A.C * size + 16383) / 16384;
+  long long want = (1024 + A.B - 1) / A.B;
+  long long S = by_bytes < want ? by_bytes : want;
+  if (S > (A.HW + 15) / 16) S = (A.HW + 15) / 16;
+  if (S > 256) S = 256;
+  if (S < 1) S = 1;
+  A.slice = (int)((A.HW + S - 1) / S);
+  A.S = (A.HW + A.slice - 1) / A.slice;
+}
+
+template <typename T, int V, int ACT>
+int forward(NormArgs& A, hipStream_t st) {
+  if (one_launch(A, sizeof(T))) {
+    const size_t lds = (lds_floats(A.range, V) + 2 * (A.range / A.per)) * sizeof(float);
+    hipLaunchKernelGGL((gna_forward_kernel<T, V, ACT>), dim3(A.B * (A.C / A.range)), dim3(kThreads), lds, st, A);
+    return (int)hipGetLastError();
+  }
+  hipLaunchKernelGGL((gna_stats_kernel<T, V>), dim3(A.B * A.S), dim3(kThreads), lds_floats(A.C, V) * sizeof(float), st, A);
+  hipLaunchKernelGGL((gna_apply_kernel<T, V, ACT>), dim3(A.B * A.S), dim3(kThreads), (size_t)A.G * 2 * sizeof(float), st, A, A.slice, A.S);
+  return (int)hipGetLastError();
+}
+
+template <typename T, int V, int ACT>
+int backward(NormArgs& A, hipStream_t st) {
+  const int param_blocks = A.dw || A.db ? (A.C + 15) / 16 : 0;
+  if (one_launch(A, sizeof(T))) {
+    A.S = 1;
+    const size_t lds = (lds_floats(A.range, V) + 2 * (A.range / A.per)) * sizeof(float);
+    hipLaunchKernelGGL((gna_backward_kernel<T, V, ACT>), dim3(A.B * (A.C / A.range)), dim3(kThreads), lds, st, A);
+    if (param_blocks) hipLaunchKernelGGL(gna_param_kernel, dim3(param_blocks), dim3(kThreads), 0, st, A);
+    return (int)hipGetLastError();
+  }
+  hipLaunchKernelGGL((gna_grad_partial_kernel<T, V, ACT>), dim3(A.B * A.S), dim3(kThreads), lds_floats(A.C, V) * sizeof(float), st, A);
+  const size_t lds = (size_t)(A.G * 2 > 512 ? A.G * 2 : 512) * sizeof(float);
+  hipLaunchKernelGGL((gna_grad_apply_kernel<T, V, ACT>), dim3(param_blocks + A.B * A.S), dim3(kThreads), lds, st, A, A.slice, A.S, param_blocks);
+  return (int)hipGetLastError();
+}
+
+template <typename T, int V>
+int by_act(NormArgs& A, int act_, bool back, hipStream_t st) {
+  switch (act_) {
+    case ACT_NONE: return back ? backward<T, V, ACT_NONE>(A, st) : forward<T, V, ACT_NONE>(A, st);
+    case ACT_RELU: return back ? backward<T, V, ACT_RELU>(A, st) : forward<T, V, ACT_RELU>(A, st);
+    case ACT_SILU: return back ? backward<T, V, ACT_SILU>(A, st) : forward<T, V, ACT_SILU>(A, st);
+    default: return back ? backward<T, V, ACT_GELU>(A, st) : forward<T, V, ACT_GELU>(A, st);
+  }
+}
+
+template <typename T>
+int by_width(NormArgs& A, int act_, bool back, uintptr_t all, hipStream_t st) {
+  const int V = vector_of(A.C, sizeof(T), all);
+  A.range = channel_range(A.C, A.G, V, sizeof(T));
+  choose_slices(A, sizeof(T));
+  switch (V) {
+    case 8: if constexpr (sizeof(T) == 2) return by_act<T, 8>(A, act_, back, st); break;
+    case 4: return by_act<T, 4>(A, act_, back, st);
+    case 2: return by_act<T, 2>(A, act_, back, st);
+    default: return by_act<T, 1>(A, act_, back, st);
+  }
+  return COMBO_EINVAL;
+}
+
+int run(NormArgs& A, int dtype, int act_, bool back, uintptr_t all, hipStream_t st) {
+  if (dtype == 0) return by_width<float>(A, act_, back, all, st);
+  if (dtype == 1) return by_width<__bf16>(A, act_, back, all, st);
+  return by_width<_Float16>(A, act_, back, all, st);
+}
+
+bool shape_ok(int B, int HW, int C, int G, int dtype, int act_) {
+  return B > 0 && HW > 0 && C > 0 && C <= kMaxC && G > 0 && C % G == 0 && dtype >= 0 && dtype <= 2 && act_ >= 0 && act_ <= 3 &&
+         (long long)B * C < 0x7fffffffll && B <= (1 << 22);
+}
+
+}  // namespace
+
+extern "C" {
+
+long long combo_groupnorm_act_workspace(int B, int HW, int C, int G, int dtype, int backward_pass) {
+  if (!shape_ok(B, HW, C, G, dtype, 0)) return -1;
+  NormArgs A = {};
+  A.B = B, A.HW = HW, A.C = C, A.G = G;
+  choose_slices(A, dtype == 0 ? 4 : 2);
+  const long long rows = (long long)B * A.S;
+  return rows * G * 2 + (backward_pass ? rows * C * 2 : 0);
+}
+
+int combo_groupnorm_act_forward(const void* x, const float* weight, const float* bias, int B, int HW, int C, int G, float eps, int act_,
+                                int dtype, float* workspace, float* mean, float* rstd, void* y, combo_stream_t stream) {
+  if (!x || !workspace || !mean || !rstd || !y || !shape_ok(B, HW, C, G, dtype, act_)) return COMBO_EINVAL;
+  const uintptr_t all = (uintptr_t)x | (uintptr_t)y;
+  if (all & (dtype == 0 ? 3 : 1)) return COMBO_EINVAL;
+  NormArgs A = {};
+  A.x = x, A.w = weight, A.bias = bias, A.mean = mean, A.rstd = rstd, A.part = workspace, A.out = y, A.eps = eps;
+  A.B = B, A.HW = HW, A.C = C, A.G = G, A.per = C / G;
+  return run(A, dtype, act_, false, all, (hipStream_t)stream);
+}
+
+int combo_groupnorm_act_backward(const void* dy, const void* x, const float* weight, const float* bias, const float* mean, const float* rstd,
+                                 int B, int HW, int C, int G, int act_, int dtype, float* workspace, void* dx, float* dweight, float* dbias,
+                                 combo_stream_t stream) {
+  if (!dy || !x || !mean || !rstd || !workspace || !dx || !shape_ok(B, HW, C, G, dtype, act_)) return COMBO_EINVAL;
+  const uintptr_t all = (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx;
+  if (all & (dtype == 0 ? 3 : 1)) return COMBO_EINVAL;
+  NormArgs A = {};
+  A.x = x, A.dy = dy, A.w = weight, A.bias = bias, A.mean = const_cast<float*>(mean), A.rstd = const_cast<float*>(rstd), A.part = workspace;
+  A.out = dx, A.dw = dweight, A.db = dbias;
+  A.B = B, A.HW = HW, A.C = C, A.G = G, A.per = C / G;
+  return run(A, dtype, act_, true, all, (hipStream_t)stream);
+}
+
+}  // extern "C"

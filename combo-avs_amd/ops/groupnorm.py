@@ -53,3 +53,101 @@ class _GroupNormNHWC(Function):
 def group_norm(x, gn, relu=False):
     """x: channels_last fp32 [B,C,H,W]; gn: nn.GroupNorm -> channels_last output (ReLU fused when asked)."""
     return _GroupNormNHWC.apply(x, gn.weight, gn.bias, gn.num_groups, gn.eps, relu)
+
+
+# ---- group norm with an activation, any of the float types and any channel count (csrc/groupnorm_act.hip) ----
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+MAX_CHANNELS = 4096
+
+
+def _channels_last(x):
+    return torch.channels_last if x.dim() == 4 else torch.channels_last_3d
+
+
+def _act_workspace(x, groups, code, backward):
+    n = _lib.lib().combo_groupnorm_act_workspace(x.shape[0], x.shape[2:].numel(), x.shape[1], groups, code, 1 if backward else 0)
+    return torch.empty(n, device=x.device, dtype=torch.float32)
+
+
+def _act_forward(x, weight, bias, groups, eps, act):
+    B, C = x.shape[:2]
+    y = torch.empty_like(x)  # (preserves channels_last)
+    stats = torch.empty(2, B, groups, device=x.device, dtype=torch.float32)
+    if x.numel() == 0:
+        return y, stats
+    code, base = _lib.FLOAT_TYPES[x.dtype], stats.data_ptr()
+    with _lib.device_of(x) as stream:
+        ws = _act_workspace(x, groups, code, False)
+        _lib.check(_lib.lib().combo_groupnorm_act_forward(x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), B, x.shape[2:].numel(), C, groups,
+                                                          eps, act, code, ws.data_ptr(), base, base + 4 * B * groups, y.data_ptr(), stream),
+                   "combo_groupnorm_act_forward")
+    return y, stats
+
+
+class _GroupNormAct(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        y, stats = _act_forward(x, weight, bias, groups, eps, act)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        B, C = x.shape[:2]
+        dx = torch.empty_like(x)
+        new = torch.zeros if x.numel() == 0 else torch.empty
+        dw = new(C, device=x.device, dtype=torch.float32) if weight is not None and ctx.needs_input_grad[1] else None
+        db = new(C, device=x.device, dtype=torch.float32) if bias is not None and ctx.needs_input_grad[2] else None
+        if x.numel() == 0:
+            return dx, dw, db, None, None, None
+        dy = dy.contiguous(memory_format=_channels_last(x))
+        code, base = _lib.FLOAT_TYPES[x.dtype], stats.data_ptr()
+        with _lib.device_of(x) as stream:
+            ws = _act_workspace(x, ctx.groups, code, True)
+            _lib.check(_lib.lib().combo_groupnorm_act_backward(dy.data_ptr(), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), base,
+                                                               base + 4 * B * ctx.groups, B, x.shape[2:].numel(), C, ctx.groups, ctx.act, code,
+                                                               ws.data_ptr(), dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), stream),
+                       "combo_groupnorm_act_backward")
+        return dx, dw, db, None, None, None
+
+
+def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none"):
+    """act(GroupNorm(x)) in one op: x [B, C, H, W] channels_last or [B, C, T, H, W] channels_last_3d in fp32, bf16 or fp16, any C that
+    `groups` divides (at most 4096) -> the same layout and type; statistics and arithmetic in fp32, rounded once.  weight, bias [C] (fp32 or
+    x's type, nullable); activation: "none", "relu", "silu", "gelu" (erf form).  Differentiable in x, weight and bias; the backward
+    pass keeps x and the statistics only."""
+    if x.dim() not in (4, 5):
+        raise ValueError(f"group_norm_act: x must be [B, C, H, W] or [B, C, T, H, W], got {tuple(x.shape)}")
+    C = x.shape[1]
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"group_norm_act: activation {activation!r}, takes one of {sorted(ACTIVATIONS)}")
+    if x.dtype not in _lib.FLOAT_TYPES:
+        raise TypeError(f"group_norm_act: x is {x.dtype}, takes float32, bfloat16 or float16")
+    if groups < 1 or C < 1 or C % groups or C > MAX_CHANNELS:
+        raise ValueError(f"group_norm_act: {C} channels in {groups} groups (the groups divide the channels, at most {MAX_CHANNELS})")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None:
+            if tuple(p.shape) != (C,):
+                raise ValueError(f"group_norm_act: {name} must be [{C}], got {tuple(p.shape)}")
+            if p.dtype not in (torch.float32, x.dtype):
+                raise TypeError(f"group_norm_act: {name} is {p.dtype}, takes float32 or x's type {x.dtype}")
+            if p.device != x.device:
+                raise ValueError(f"group_norm_act: {name} is on {p.device}, x on {x.device}")
+    if not x.is_contiguous(memory_format=_channels_last(x)):
+        raise ValueError("group_norm_act: x must be channels-last (x.contiguous(memory_format=torch.channels_last), _3d for five dimensions)")
+    if x.shape[2:].numel() >= 1 << 31:
+        raise ValueError("group_norm_act: more than 2^31 places in a map")
+    if not x.is_cuda:
+        raise RuntimeError("combo_avs_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
+    if weight is not None:
+        weight = weight.float().contiguous()
+    if bias is not None:
+        bias = bias.float().contiguous()
+    args = (x, weight, bias, int(groups), float(eps), ACTIVATIONS[activation])
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _GroupNormAct.apply(*args)
+    return _act_forward(*args)[0]

@@ -663,6 +663,34 @@ int combo_adamw_f32(float* param, const float* grad, float* exp_avg, float* exp_
                     const float* clip_coef, float lr, float weight_decay, float beta1, float beta2, float eps,
                     float bias_correction1, float bias_correction2, combo_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Group norm with an activation on channels-last maps [B,HW,C], any C that G divides (C <= 4096)
+ *   y = act((x - mean) rstd weight + bias), act 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf); x, y, dy, dx of `dtype` (0 fp32, 1 bf16, 2 fp16),
+ *   weight / bias fp32 (NULL: 1 / 0).  mean, rstd [B,G]: written by the forward pass, read by the backward pass.
+ *   workspace: combo_groupnorm_act_workspace floats (-1: shape refused), not shared by calls that may run at the same time.
+ *   dweight, dbias [C] fp32 (NULL: not wanted).  All sums in a fixed order.
+ * ---------------------------------------------------------------------------------------------- */
+long long combo_groupnorm_act_workspace(int B, int HW, int C, int G, int dtype, int backward_pass);
+int combo_groupnorm_act_forward(const void* x, const float* weight, const float* bias, int B, int HW, int C, int G, float eps, int act,
+                                int dtype, float* workspace, float* mean, float* rstd, void* y, combo_stream_t stream);
+int combo_groupnorm_act_backward(const void* dy, const void* x, const float* weight, const float* bias, const float* mean,
+                                 const float* rstd, int B, int HW, int C, int G, int act, int dtype, float* workspace, void* dx,
+                                 float* dweight, float* dbias, combo_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Rotary positions over several axes
+ *   x [B,N,H,D] (strides in elements, last dimension contiguous) -> y [B,N,H,D] contiguous, both of `dtype` (0 fp32, 1 bf16, 2 fp16).
+ *   sections_host[a]: pairs of axis a, P = their sum <= D/2; turns_host[P]: frequency of every pair / 2 pi.  Pair j = the values
+ *   (j, j+P), interleaved != 0: (2j, 2j+1), is turned by 2 pi turns_host[j] * position[axis(j)] (inverse != 0: backwards, which is
+ *   the gradient); values from 2P on are copied.  positions: (b, n, a) strides in elements, position_type 0 fp32, 1 fp64, 2 int32,
+ *   3 int64.  D even, <= 256; axes <= 8.  interleaved: the strides of x are even and x, y are aligned to a pair.
+ *   The two host arrays are read before the call returns.
+ * ---------------------------------------------------------------------------------------------- */
+int combo_rotary_axes(const void* x, long long stride_b, long long stride_n, long long stride_h, int dtype, const void* positions,
+                      int position_type, long long pos_stride_b, long long pos_stride_n, long long pos_stride_axis, int B, int N,
+                      int H, int D, int axes, const int* sections_host, const double* turns_host, int interleaved, int inverse,
+                      void* y, combo_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
