@@ -132,6 +132,10 @@ _SIGNATURES = {
     "combo_attention_backward_f32": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p] + [c_int] * 5 + [c_float] + [c_void_p] * 8,
     "combo_attention_backward_ld_f32": [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_void_p] + [c_int] * 5 + [c_float]
                                        + [c_void_p] * 6 + [c_longlong, c_void_p, c_longlong, c_void_p],
+    "combo_cross_attention_workspace": [c_void_p, c_int],
+    "combo_cross_attention_forward": [c_void_p] * 5,
+    "combo_cross_attention_backward": [c_void_p] * 9,
+    "combo_cross_attention_pack": [c_void_p] + [c_longlong] * 4 + [c_int] * 4 + [c_void_p, c_void_p],
     "combo_groupnorm_act_workspace": [c_int] * 6,
     "combo_groupnorm_act_forward": [c_void_p] * 3 + [c_int] * 4 + [c_float, c_int, c_int] + [c_void_p] * 5,
     "combo_groupnorm_act_backward": [c_void_p] * 6 + [c_int] * 6 + [c_void_p] * 5,
@@ -144,7 +148,7 @@ _SIGNATURES = {
     "combo_sra_attention_backward_bf16": [c_void_p] * 9 + [c_int] * 4 + [c_float, c_void_p],
 }
 _RESTYPES = {"combo_build_arch": ctypes.c_char_p, "combo_sra_attention_backward_workspace": ctypes.c_longlong,
-             "combo_groupnorm_act_workspace": ctypes.c_longlong}
+             "combo_groupnorm_act_workspace": ctypes.c_longlong, "combo_cross_attention_workspace": ctypes.c_longlong}
 
 
 def exported_symbols():
@@ -196,6 +200,29 @@ def current_stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+
+
+_LEAF_MARK = "combo_avs_default_stream"
+
+
+def record(function, *args):
+    """function.apply(*args).  Autograd keeps ONE accumulation node per leaf, alive as long as any graph of the leaf, and that node remembers
+    the stream on which it was made.  If that is the default stream, a backward pass that is captured into a graph has to join it,
+    which ends the process when the capture does: so an eager call on the default stream marks the nodes of its leaves, and a call inside a
+    capture that finds a marked node alive refuses."""
+    import torch
+    if torch.cuda.is_current_stream_capturing():
+        for t in args:
+            if torch.is_tensor(t) and t.requires_grad and t.is_leaf and _LEAF_MARK in torch.autograd.graph.get_gradient_edge(t).node.metadata:
+                raise RuntimeError("a graph is being captured while an eager autograd graph of the same leaf, recorded on the default stream, is "
+                                   "alive: drop its outputs (or detach them) before the capture, or record them on another stream")
+        return function.apply(*args)
+    out = function.apply(*args)
+    if current_stream() == 0:
+        for node, _ in out.grad_fn.next_functions:
+            if type(node).__name__ == "AccumulateGrad":
+                node.metadata[_LEAF_MARK] = True
+    return out
 
 
 class device_of:

@@ -149,5 +149,5 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
         bias = bias.float().contiguous()
     args = (x, weight, bias, int(groups), float(eps), ACTIVATIONS[activation])
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _GroupNormAct.apply(*args)
+        return _lib.record(_GroupNormAct, *args)
     return _act_forward(*args)[0]

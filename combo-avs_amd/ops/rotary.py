@@ -89,7 +89,7 @@ def rotary_axes(x, positions, sections, base=10000.0, interleaved=False, shared_
         raise RuntimeError("combo_avs_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
     how = (sections, base, bool(interleaved), bool(shared_ladder))
     if x.requires_grad and torch.is_grad_enabled():
-        return _Rotary.apply(x, positions, how)
+        return _lib.record(_Rotary, x, positions, how)
     return _rotate(x, positions, *how, False)
 
 

@@ -664,6 +664,36 @@ int combo_adamw_f32(float* param, const float* grad, float* exp_avg, float* exp_
                     float bias_correction1, float bias_correction2, combo_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Cross attention of queries to encoder states of another length (bf16 / fp16, grouped heads, lengths, mask)
+ *   out[b,n,h] = sum_j softmax_j(scale q[b,n,h] . k[b,j,h / (Hq/Hk)]) v[b,j,h / (Hq/Hk)] over the keys j < kv_lengths[b] whose bit is
+ *   clear; a row without an open key gives zeros and passes no gradient.  States behind a sample's length, and states blocked by a mask
+ *   that all queries share (bits_stride[2] == 0 and the heads of a group share it), are never part of a product, whatever they hold.
+ *   q [B,Lq,Hq,D], k / v [B,Lk,Hk,D]: strides (batch, token, head) in elements, multiples of 8, the last dimension contiguous, pointers
+ *   16-byte aligned.  Hk divides Hq, D % 8 == 0, D <= 128, scale > 0.  dtype 1 bf16, 2 fp16.
+ *   kv_lengths [B] (nullable; clamped to 0 .. Lk).  blocked_bits (nullable): word w of a line holds the keys 32 w .. 32 w + 31, 1 = blocked;
+ *   bits_stride: (batch, query head, query) in words, 0 where shared; combo_cross_attention_pack writes it from a byte (bool) mask
+ *   [B,H,N,Lk] with strides in bytes into [B,H,N,(Lk+31)/32].
+ *   out, dout, dq [B,Lq,Hq,D], dk, dv [B,Lk,Hk,D] (both or neither) contiguous, 16-byte aligned.  lse [B*Hk*Lq*Hq/Hk] fp32: written by the forward pass
+ *   (NULL: not wanted), read by the backward pass.  workspace: combo_cross_attention_workspace bytes (-1: refused; 0: none needed in the
+ *   forward pass), 32-byte aligned, not shared by calls that may run at the same time.  All sums in a fixed order.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct combo_cross_attention {
+  const void *q, *k, *v;
+  long long q_stride[3], k_stride[3], v_stride[3];
+  const int* kv_lengths;
+  const unsigned* blocked_bits;
+  long long bits_stride[3];
+  int B, Lq, Lk, Hq, Hk, D, dtype;
+  float scale;
+} combo_cross_attention_t;
+long long combo_cross_attention_workspace(const combo_cross_attention_t* desc_host, int backward_pass);
+int combo_cross_attention_forward(const combo_cross_attention_t* desc_host, void* out, float* lse, void* workspace, combo_stream_t stream);
+int combo_cross_attention_backward(const combo_cross_attention_t* desc_host, const void* out, const float* lse, const void* dout,
+                                   void* workspace, void* dq, void* dk, void* dv, combo_stream_t stream);
+int combo_cross_attention_pack(const unsigned char* blocked, long long stride_b, long long stride_h, long long stride_n, long long stride_k,
+                               int B, int H, int N, int Lk, unsigned* bits, combo_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Group norm with an activation on channels-last maps [B,HW,C], any C that G divides (C <= 4096)
  *   y = act((x - mean) rstd weight + bias), act 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf); x, y, dy, dx of `dtype` (0 fp32, 1 bf16, 2 fp16),
  *   weight / bias fp32 (NULL: 1 / 0).  mean, rstd [B,G]: written by the forward pass, read by the backward pass.

@@ -1,4 +1,4 @@
-"""CPU: what the entry points of group norm with an activation and rotary positions refuse, before anything is launched."""
+"""CPU: what the entry points of group norm with an activation, rotary positions and cross attention refuse, before anything is launched."""
 import pytest
 import torch
 
@@ -53,3 +53,46 @@ def test_entry_points_refuse_bad_arguments_without_a_launch():
     assert lib.combo_groupnorm_act_forward(one, 0, 0, 1, 9, 8, 2, 1e-5, 4, 0, one, one, one, one, 0) == 1
     assert lib.combo_groupnorm_act_forward(one + 2, 0, 0, 1, 9, 8, 2, 1e-5, 0, 0, one, one, one, one, 0) == 1
     assert lib.combo_groupnorm_act_backward(0, one, 0, 0, one, one, 1, 9, 8, 2, 0, 0, one, one, 0, 0, 0) == 1
+
+
+def test_cross_attention_refusals():
+    from combo_avs_amd.ops.cross_attention import cross_attention
+    q, k = torch.zeros(2, 3, 4, 16).half(), torch.zeros(2, 5, 2, 16).half()
+    n = torch.tensor([1, 2], dtype=torch.int32)
+    for bad in (lambda: cross_attention(q[0], k, k), lambda: cross_attention(q, k, k[:, :4]), lambda: cross_attention(q[:1], k, k),
+                lambda: cross_attention(q, k[..., :8], k[..., :8]), lambda: cross_attention(q[..., :12], k[..., :12], k[..., :12]),
+                lambda: cross_attention(q[:, :, :3], k, k), lambda: cross_attention(q, k[:, :, :0], k[:, :, :0]), lambda: cross_attention(q, k, k, scale=0.0),
+                lambda: cross_attention(q, k, k, scale=-1.0), lambda: cross_attention(q, k, k, scale=float("nan")), lambda: cross_attention(q, k, k, n[:1]),
+                lambda: cross_attention(q, k, k, blocked=torch.zeros(2, 1, 3, 4, dtype=torch.bool)),
+                lambda: cross_attention(q, k, k, blocked=torch.zeros(3, 5, dtype=torch.bool)),
+                lambda: cross_attention(q, k, k, blocked=torch.zeros(2, 2, 3, 5, dtype=torch.bool)),
+                lambda: cross_attention(torch.zeros(1, 1, 1, 136).half(), torch.zeros(1, 1, 1, 136).half(), torch.zeros(1, 1, 1, 136).half())):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: cross_attention(q.float(), k.float(), k.float()), lambda: cross_attention(q, k, k.bfloat16()), lambda: cross_attention(q, k, k, n.short()),
+                lambda: cross_attention(q, k, k, blocked=torch.zeros(2, 1, 3, 5, dtype=torch.uint8)),
+                lambda: cross_attention(q, k, k, blocked=torch.full((2, 1, 3, 5), torch.finfo(torch.float16).min))):
+        with pytest.raises(TypeError):
+            bad()
+    with pytest.raises(RuntimeError, match="GPU only"):
+        cross_attention(q, k, k, n)
+
+
+def test_cross_attention_entry_points_refuse_without_a_launch():
+    from combo_avs_amd import _lib
+    from combo_avs_amd.ops.cross_attention import _DESC
+    lib, one = _lib.lib(), 4096
+
+    def desc(q=one, qs=(64, 32, 16), B=1, Lq=2, Lk=3, Hq=2, Hk=1, D=16, dtype=1, scale=0.25):
+        return _DESC.pack(q, one, one, *qs, *qs, *qs, 0, 0, 0, 0, 0, B, Lq, Lk, Hq, Hk, D, dtype, scale)
+    assert lib.combo_cross_attention_workspace(desc(), 0) == 0 and lib.combo_cross_attention_workspace(desc(), 1) >= 16
+    for bad in (desc(q=0), desc(q=one + 2), desc(qs=(64, 32, 12)), desc(qs=(64, -32, 16)), desc(B=0), desc(Lq=0), desc(Lk=0), desc(Hk=3), desc(D=12),
+                desc(D=136), desc(dtype=0), desc(dtype=3), desc(scale=0.0), desc(scale=float("inf")), desc(scale=float("nan")), desc(Lq=1 << 30),
+                desc(B=1 << 24)):
+        assert lib.combo_cross_attention_workspace(bad, 0) == -1
+        assert lib.combo_cross_attention_forward(bad, one, 0, one, 0) == 1
+        assert lib.combo_cross_attention_backward(bad, one, one, one, one, one, one, one, 0) == 1
+    assert lib.combo_cross_attention_forward(desc(), 0, 0, one, 0) == 1 and lib.combo_cross_attention_forward(desc(), one + 8, 0, one, 0) == 1
+    assert lib.combo_cross_attention_forward(desc(Lk=1000), one, 0, 0, 0) == 1  # split keys need their workspace
+    assert lib.combo_cross_attention_backward(desc(), one, one, one, one, one, one, 0, 0) == 1  # dk without dv
+    assert lib.combo_cross_attention_pack(one, 1, 1, 1, 1, 0, 1, 1, 1, one, 0) == 1
