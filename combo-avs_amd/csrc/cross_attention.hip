@@ -9,8 +9,9 @@
 // one row - the softmax statistics are lane-local plus one exchange with the other half wave - and the tile is, register for register, the B
 // operand of the product that follows when that product's contraction runs in the order in which a lane holds its keys (4 h + 0..3,
 // 8 + 4 h + 0..3 of every 16).  The A operand in that order is the transpose of a row-major LDS tile: ds_read_b64_tr_b16 reads it, so K, V, Q
-// and dO are each staged once, row-major, for both uses.  LDS tiles are swizzled in 16-byte chunks (Tile::chunk).
+// and dO are each staged once, row-major, for both uses.  LDS tiles are padded (Tile).
 #include <cmath>
+#include <type_traits>
 
 #include "combo_common.h"
 
@@ -61,19 +62,14 @@ __device__ __forceinline__ int length_of(const Args& A, int b) {
   return A.lens ? min(max(A.lens[b], 0), A.Lk) : A.Lk;
 }
 
-// row-major LDS tile of 16-bit values, DP a row, in chunks of 8: chunk c of row r lies at chunk c ^ swizzle(r).  16 rows at the same chunk
-// (a b128 operand read) and 4 rows x 4 neighbouring chunks (a transposed read) then both spread over all banks: the swizzle is the bit
-// reversal of the row's index among those that start at the same bank.
+// row-major LDS tile of 16-bit values.  The pitch is an odd number p of 16-byte chunks with p = 3, 7 or 9 (mod 16): 16 rows at the same chunk (a
+// b128 operand read) start in 16 different chunks of the 64 banks, and 4 rows x 2 neighbouring chunks (16 lanes of a transposed read) in 8, so
+// neither conflicts (SQ_LDS_BANK_CONFLICT: 0), and every address is one lane register plus an immediate; a swizzle by exclusive-or costs a
+// register or an instruction per operand, and the kernels are short of both.
 template <int DP>
 struct Tile {
-  static constexpr int CH = DP / 8, PER = 16 / CH;  // chunks of a row; rows over which the banks repeat
-  static __device__ __forceinline__ int swizzle(int r) {
-    const int x = (r / PER) & (CH - 1);
-    if constexpr (CH == 4) return x;
-    if constexpr (CH == 8) return ((x & 1) << 2) | (x & 2) | ((x >> 2) & 1);
-    return ((x & 1) << 3) | ((x & 2) << 1) | ((x & 4) >> 1) | ((x >> 3) & 1);
-  }
-  static __device__ __forceinline__ int at(int r, int c) { return r * DP + ((c ^ swizzle(r)) << 3); }
+  static constexpr int PITCH = DP == 32 ? 56 : (DP == 64 ? 72 : 152);
+  static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + c * 8; }
 };
 
 // A (or B) operand of a product over the row's own dimension: row r0 + (lane & 31), values 16 step + 8 half .. + 7
@@ -89,8 +85,8 @@ __device__ __forceinline__ typename Type<T>::x8 operand_t(const T* tile, int r0,
   const int lane = threadIdx.x & 63, row = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
   const int col = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   typedef __attribute__((address_space(3))) s16x4 lds4;
-  const T* a = tile + Tile<DP>::at(row, col >> 3) + (col & 7);
-  const T* b = tile + Tile<DP>::at(row + 8, col >> 3) + (col & 7);
+  const T* a = tile + row * Tile<DP>::PITCH + col;
+  const T* b = a + 8 * Tile<DP>::PITCH;
   const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)a), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)b);
   return __builtin_bit_cast(typename Type<T>::x8, (s16x8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
 }
@@ -116,29 +112,43 @@ __device__ __forceinline__ float both_sum(float x) {
 // index of register i of a 32 x 32 result along its rows
 __device__ __forceinline__ int reg_row(int i, int half) { return 8 * (i >> 2) + 4 * half + (i & 3); }
 
-// ROWS rows of DP values from global memory into registers and on into an LDS tile; rows from `valid` on, chunks from D on and rows whose bit
-// is set in `skip` (blocked for every query: whatever such a state holds never meets a product) become zeros
+// ROWS rows of DP values from global memory into registers and on into an LDS tile.  A thread's place in the tile does not change from tile to
+// tile: `at` (bytes from the tile's first row; one add per tile is left, of a uniform pointer) and `to` (LDS) are computed once, and its N
+// vectors lie a fixed number of rows apart.  Rows from `valid` on, chunks from D on and rows whose bit is
+// set in `skip` (blocked for every query: whatever such a state holds never meets a product) become zeros.
 template <typename T, int DP, int ROWS>
 struct Stage {
-  static constexpr int N = ROWS * (DP / 8) / 256;
+  static constexpr int N = ROWS * (DP / 8) / 256, STEP = 256 / (DP / 8);
   u32x4 r[N];
-  __device__ __forceinline__ void load(const T* base, long long stride, int row0, int valid, int D, const unsigned* skip) {
+  unsigned at;
+  int row, to;
+  bool chunk;
+  __device__ __forceinline__ void place(long long stride, int D) {
+    const int c = threadIdx.x % (DP / 8);
+    row = threadIdx.x / (DP / 8);
+    at = (unsigned)(row * (int)stride + c * 8) * 2u;
+    to = Tile<DP>::at(row, c);
+    chunk = c * 8 < D;
+  }
+  // tile: address of the tile's first row; step: bytes of STEP rows; valid: rows the tile has; whole: all of it is loaded
+  __device__ __forceinline__ void load(const char* tile, long long step, int valid, bool whole, const unsigned* skip, int row0) {
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int x = threadIdx.x + 256 * i, row = row0 + x / (DP / 8), c = x % (DP / 8);
-      bool on = row < valid && c * 8 < D;
-      if (skip && on) on = !((skip[row >> 5] >> (row & 31)) & 1);
-      u32x4 z = {0u, 0u, 0u, 0u};
-      if (on) z = *reinterpret_cast<const u32x4*>(base + row * stride + c * 8);
-      r[i] = z;
+      for (int i = 0; i < N; ++i) r[i] = *reinterpret_cast<const u32x4*>(tile + i * step + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int x = row + STEP * i;
+        bool on = chunk && x < valid;
+        if (skip && on) on = !((skip[(row0 + x) >> 5] >> ((row0 + x) & 31)) & 1);
+        r[i] = u32x4{0u, 0u, 0u, 0u};
+        if (on) r[i] = *reinterpret_cast<const u32x4*>(tile + i * step + at);
+      }
     }
   }
   __device__ __forceinline__ void store(T* tile) const {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int x = threadIdx.x + 256 * i, row = x / (DP / 8), c = x % (DP / 8);
-      *reinterpret_cast<u32x4*>(tile + Tile<DP>::at(row, c)) = r[i];
-    }
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(tile + to + i * STEP * Tile<DP>::PITCH) = r[i];
   }
 };
 
@@ -185,169 +195,312 @@ __device__ __forceinline__ Range split_range(int len, int splits, int s, int til
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------
 
-// RW waves along the rows (32 each), 4 / RW along the keys of a tile
-template <typename T, int DP, int RW>
-struct Fwd {
-  static constexpr int KW = 4 / RW, KB = RW == 4 ? 2 : 1, KT = 32 * KB * KW, RT = 32 * RW;
-  static constexpr int LDS = 2 * KT * DP * 2 + (KW > 1 ? 2 * KW * 32 * 4 : 0);
-  static_assert(KW == 1 || KW * 32 * DP * 4 <= 2 * KT * DP * 2, "the join of the key waves fits the tiles");
+// few rows (at most 32): the four waves hold the same rows and share the keys of a tile, 32 each
+template <int DP>
+struct Few {
+  static constexpr int KW = 4, KT = 32 * KW, TILE = KT * Tile<DP>::PITCH;
+  static constexpr int LDS = 2 * TILE * 2 + 2 * KW * 32 * 4;
+  static_assert(KW * 32 * DP * 4 <= 2 * TILE * 2, "the join of the waves fits the tiles");
 };
 
-template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(256) cross_forward_kernel(const Args A) {
-  typedef Fwd<T, DP, RW> F;
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 x;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = 0.f;
+  return x;
+}
+
+// running softmax of one row block: raw maximum m (of the scores before scaling), sum l of this lane's keys
+struct Running {
+  float m = -kInf, l = 0.f;
+  __device__ __forceinline__ float base(float c) const { return m == -kInf ? 0.f : m * c; }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, 2) cross_few_kernel(const Args A) {
+  typedef Few<DP> F;
   typedef typename Type<T>::x8 x8;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* Kt = reinterpret_cast<T*>(lds);
-  T* Vt = Kt + F::KT * DP;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int rw = wave % RW, kw = wave / RW;
+  T* Vt = Kt + F::TILE;
+  const int lane = threadIdx.x & 63, kw = threadIdx.x >> 6, half = lane >> 5, r = lane & 31;
   int id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int tile = id % A.tiles;
-  id /= A.tiles;
   const int split = id % A.splits;
   id /= A.splits;
-  const int hk = id % A.Hk, b = id / A.Hk;
-  const int r = tile * F::RT + rw * 32 + (lane & 31), len = length_of(A, b);
+  const int hk = id % A.Hk, b = id / A.Hk, len = length_of(A, b);
   const Row row(A, hk, min(r, A.rows - 1));
   const Range keys = split_range(len, A.splits, split, F::KT);
-  const T* k = reinterpret_cast<const T*>(A.k) + b * A.kb + hk * A.kh;
-  const T* v = reinterpret_cast<const T*>(A.v) + b * A.vb + hk * A.vh;
+  const char* k = A.k + 2 * (b * A.kb + hk * A.kh);
+  const char* v = A.v + 2 * (b * A.vb + hk * A.vh);
   const unsigned* words = A.bits ? A.bits + b * A.mb + row.h * A.mh + row.n * A.mn : nullptr;
   const unsigned* skip = A.bits && A.mn == 0 && (A.mh == 0 || A.G == 1) ? A.bits + b * A.mb + hk * A.mh : nullptr;
   x8 q[DP / 16];
   row_operand<T, DP>(reinterpret_cast<const T*>(A.q) + b * A.qb + row.n * A.qn + row.h * A.qh, A.D, r < A.rows, q);
   f32x16 acc[DP / 32];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
-  float m = -kInf, l = 0.f;
+  for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
+  Running run;
   Stage<T, DP, F::KT> sk, sv;
+  sk.place(A.kn, A.D);
+  sv.place(A.vn, A.D);
+  const bool all = A.D == DP && !skip;
+  auto fetch = [&](int k0) {
+    const bool whole = all && k0 + F::KT <= len;
+    sk.load(k + 2 * k0 * A.kn, 2 * sk.STEP * A.kn, len - k0, whole, skip, k0);
+    sv.load(v + 2 * k0 * A.vn, 2 * sv.STEP * A.vn, len - k0, whole, skip, k0);
+  };
+  if (keys.lo < keys.hi) fetch(keys.lo);
   for (int k0 = keys.lo; k0 < keys.hi; k0 += F::KT) {
-    sk.load(k, A.kn, k0, len, A.D, skip);
-    sv.load(v, A.vn, k0, len, A.D, skip);
     __syncthreads();
     sk.store(Kt);
     sv.store(Vt);
+    if (k0 + F::KT < keys.hi) fetch(k0 + F::KT);  // the next tile travels while this one is multiplied
     __syncthreads();
-    f32x16 s[F::KB];
+    f32x16 s;
 #pragma unroll
-    for (int kb = 0; kb < F::KB; ++kb) {
-      const int row0 = (kw * F::KB + kb) * 32;
+    for (int d = 0; d < DP / 16; ++d) s = Type<T>::mfma(operand<T, DP>(Kt, 32 * kw, d), q[d], d ? s : zero16());
+    if (A.bits || k0 + F::KT > len) mask_scores(s, k0 + 32 * kw, len, words, half);
+    float top = run.m;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) s[kb] = Type<T>::mfma(operand<T, DP>(Kt, row0, d), q[d], s[kb]);
-      mask_scores(s[kb], k0 + row0, len, words, half);
-    }
-    float top = m;
-#pragma unroll
-    for (int kb = 0; kb < F::KB; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
     top = other_max(top);
-    const float base = top == -kInf ? 0.f : top * A.c;
-    const float alpha = __builtin_amdgcn_exp2f(m * A.c - base);  // (m = -inf: 0)
-    m = top;
-    l *= alpha;
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
-#pragma unroll
-    for (int kb = 0; kb < F::KB; ++kb) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], A.c, -base));
-        l += s[kb][i];
-      }
-      // p is rounded to the tensor's type for the product (half a step relative to each p); its sum l keeps 32 bits
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const x8 p = pack<T>(s[kb], st);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mfma(operand_t<T, DP>(Vt, (kw * F::KB + kb) * 32 + 16 * st, 32 * d), p, acc[d]);
-      }
-    }
-  }
-  l = both_sum(l);
-  float lse;
-  if constexpr (F::KW > 1) {  // the key waves hold the same rows: join their maxima, sums and results
-    float* ml = reinterpret_cast<float*>(lds + 2 * F::KT * DP * 2);
-    float* part = reinterpret_cast<float*>(lds);  // [KW][DP][32]
-    __syncthreads();
-    if (half == 0) {
-      ml[kw * 32 + lane] = m;
-      ml[(F::KW + kw) * 32 + lane] = l;
-    }
-    __syncthreads();
-    float top = -kInf, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < F::KW; ++w) top = fmaxf(top, ml[w * 32 + (lane & 31)]);
-    const float base = top == -kInf ? 0.f : top * A.c;
-#pragma unroll
-    for (int w = 0; w < F::KW; ++w)
-      sum += ml[(F::KW + w) * 32 + (lane & 31)] * __builtin_amdgcn_exp2f(ml[w * 32 + (lane & 31)] * A.c - base);
-    const float f = sum > 0.f ? __builtin_amdgcn_exp2f(m * A.c - base) / sum : (sum == 0.f ? 0.f : sum);
-    lse = sum > 0.f ? base + log2f(sum) : (sum == 0.f ? -kInf : sum);
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) part[(kw * DP + 32 * d + reg_row(i, half)) * 32 + (lane & 31)] = acc[d][i] * f;
-    __syncthreads();
-    // wave w gathers its share of the dimensions
-    if (r < A.rows) {
-#pragma unroll
-      for (int i = 0; i < DP / 8; i += 4) {
-        const int d = (kw * 2 + half) * (DP / 8) + i;
-        float x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[j] = 0.f;
-#pragma unroll
-          for (int w = 0; w < F::KW; ++w) x[j] += part[(w * DP + d + j) * 32 + (lane & 31)];
-        }
-        if (d < A.D) {
-          if (A.splits > 1) {
-            float* o = A.part + ((((long long)split * A.B + b) * A.Hk + hk) * A.rows + r) * A.D + d;
-            *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
-          } else {
-            typename Type<T>::x4 y;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = (T)x[j];
-            *reinterpret_cast<typename Type<T>::x4*>(static_cast<T*>(A.out) + row.packed(A, b) + d) = y;
-          }
-        }
-      }
-    }
-    if (kw != 0) return;
-  } else {
-    const float base = m == -kInf ? 0.f : m * A.c;
-    const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    lse = l > 0.f ? base + log2f(l) : (l == 0.f ? -kInf : l);
-    if (r < A.rows) {
+    if (__any((top - run.m) * A.c > 8.f)) {  // as in cross_wide_kernel
+      const float to = top == -kInf ? 0.f : top * A.c;
+      const float alpha = __builtin_amdgcn_exp2f(run.m * A.c - to);
+      run.m = top;
+      run.l *= alpha;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const int dd = 32 * d + reg_row(i, half);
-          if (dd < A.D) {
-            if (A.splits > 1) {
-              float* o = A.part + ((((long long)split * A.B + b) * A.Hk + hk) * A.rows + r) * A.D + dd;
-              *reinterpret_cast<float4*>(o) = make_float4(acc[d][i] * f, acc[d][i + 1] * f, acc[d][i + 2] * f, acc[d][i + 3] * f);
-            } else {
-              typename Type<T>::x4 y;
+        for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+    }
+    const float base = run.base(A.c);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) y[j] = (T)(acc[d][i + j] * f);
-              *reinterpret_cast<typename Type<T>::x4*>(static_cast<T*>(A.out) + row.packed(A, b) + dd) = y;
-            }
-          }
-        }
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], A.c, -base));
+      run.l += s[i];
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const x8 p = pack<T>(s, st);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mfma(operand_t<T, DP>(Vt, 32 * kw + 16 * st, 32 * d), p, acc[d]);
     }
   }
-  if (half == 0 && r < A.rows) {
-    const long long at = ((long long)b * A.Hk + hk) * A.rows + r;
+  // the waves hold the same rows: join their maxima, sums and results
+  const float l = both_sum(run.l), m = run.m;
+  float* ml = reinterpret_cast<float*>(lds + 2 * F::TILE * 2);
+  float* part = reinterpret_cast<float*>(lds);  // [KW][DP][32]
+  __syncthreads();
+  if (half == 0) {
+    ml[kw * 32 + lane] = m;
+    ml[(F::KW + kw) * 32 + lane] = l;
+  }
+  __syncthreads();
+  float top = -kInf, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < F::KW; ++w) top = fmaxf(top, ml[w * 32 + r]);
+  const float base = top == -kInf ? 0.f : top * A.c;
+#pragma unroll
+  for (int w = 0; w < F::KW; ++w) sum += ml[(F::KW + w) * 32 + r] * __builtin_amdgcn_exp2f(ml[w * 32 + r] * A.c - base);
+  const float f = sum > 0.f ? __builtin_amdgcn_exp2f(m * A.c - base) / sum : (sum == 0.f ? 0.f : sum);
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) part[(kw * DP + 32 * d + reg_row(i, half)) * 32 + r] = acc[d][i] * f;
+  __syncthreads();
+  if (r >= A.rows) return;
+  const long long at = ((long long)b * A.Hk + hk) * A.rows + r, total = (long long)A.B * A.Hk * A.rows;
+  // wave w gathers its share of the dimensions
+#pragma unroll
+  for (int i = 0; i < DP / 8; i += 4) {
+    const int d = (kw * 2 + half) * (DP / 8) + i;
+    if (d >= A.D) continue;
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = 0.f;
+#pragma unroll
+      for (int w = 0; w < F::KW; ++w) x[j] += part[(w * DP + d + j) * 32 + r];
+    }
+    if (A.splits > 1) {
+      *reinterpret_cast<float4*>(A.part + (split * total + at) * A.D + d) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+      typename Type<T>::x4 y;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = (T)x[j];
+      *reinterpret_cast<typename Type<T>::x4*>(static_cast<T*>(A.out) + row.packed(A, b) + d) = y;
+    }
+  }
+  if (kw == 0 && half == 0) {
+    const float lse = sum > 0.f ? base + log2f(sum) : (sum == 0.f ? -kInf : sum);
+    if (A.splits > 1) A.part_lse[split * total + at] = lse;
+    else if (A.lse) A.lse[at] = lse == -kInf ? kInf : lse;  // (+inf: the backward pass finds p = 0)
+  }
+}
+
+// many rows: a wave owns 32, the workgroup 128.  A wave's matrix instructions and its softmax would take turns (a score costs ~5 vector
+// instructions of 4 cycles for D / 8 cycles of the matrix pipe), so three tiles are in work at once: while the vector unit turns the scores of
+// tile t into probabilities, the matrix pipe forms the scores of tile t + 1 and adds the product of tile t - 1 - in one basic block, interleaved
+// by hand.  K and V have two LDS buffers each and one barrier a tile: K runs one tile ahead, V one behind.
+template <int DP>
+struct Wide {
+  static constexpr int KB = DP == 128 ? 1 : 2, KT = 32 * KB, RT = 128, TILE = KT * Tile<DP>::PITCH;
+  static constexpr int LDS = 4 * TILE * 2;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, 2) cross_wide_kernel(const Args A) {
+  typedef Wide<DP> F;
+  typedef typename Type<T>::x8 x8;
+  constexpr int KB = F::KB;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  T* kbuf = reinterpret_cast<T*>(lds);
+  T* vbuf = kbuf + 2 * F::TILE;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  int id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int tile = id % A.tiles;
+  id /= A.tiles;
+  const int split = id % A.splits;
+  id /= A.splits;
+  const int hk = id % A.Hk, b = id / A.Hk;
+  const int r = tile * F::RT + wave * 32 + (lane & 31), len = length_of(A, b);
+  const Range keys = split_range(len, A.splits, split, F::KT);
+  const char* k = A.k + 2 * (b * A.kb + hk * A.kh);
+  const char* v = A.v + 2 * (b * A.vb + hk * A.vh);
+  const unsigned* skip = A.bits && A.mn == 0 && (A.mh == 0 || A.G == 1) ? A.bits + b * A.mb + hk * A.mh : nullptr;
+  const unsigned* words = nullptr;
+  x8 q[DP / 16];
+  {
+    const Row row(A, hk, min(r, A.rows - 1));
+    row_operand<T, DP>(reinterpret_cast<const T*>(A.q) + b * A.qb + row.n * A.qn + row.h * A.qh, A.D, r < A.rows, q);
+    if (A.bits) words = A.bits + b * A.mb + row.h * A.mh + row.n * A.mn;
+  }
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
+  Stage<T, DP, F::KT> sk, sv;
+  sk.place(A.kn, A.D);
+  sv.place(A.vn, A.D);
+  const bool all = A.D == DP && !skip;
+  const int steps = (keys.hi - keys.lo + F::KT - 1) / F::KT;
+  auto fetch_k = [&](int t) {
+    const int k0 = keys.lo + t * F::KT;
+    sk.load(k + 2 * k0 * A.kn, 2 * sk.STEP * A.kn, len - k0, all && k0 + F::KT <= len, skip, k0);
+  };
+  auto fetch_v = [&](int t) {
+    const int k0 = keys.lo + t * F::KT;
+    sv.load(v + 2 * k0 * A.vn, 2 * sv.STEP * A.vn, len - k0, all && k0 + F::KT <= len, skip, k0);
+  };
+  x8 p[KB][2];  // the probabilities of the tile before, in the order of the second product
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) p[kb][0] = p[kb][1] = pack<T>(zero16(), 0);
+  auto scores = [&](const T* Kt, f32x16 (&x)[KB]) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) x[kb] = Type<T>::mfma(operand<T, DP>(Kt, kb * 32, d), q[d], d ? x[kb] : zero16());
+  };
+  auto add_values = [&](const T* Vt) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mfma(operand_t<T, DP>(Vt, kb * 32 + 16 * st, 32 * d), p[kb][st], acc[d]);
+  };
+  Running run;
+  // tile t: its scores s; the scores of tile t + 1 go to `next`; `now`, `other`: the buffers of tile t and of its neighbours
+  auto step = [&](int t, f32x16 (&s)[KB], f32x16 (&next)[KB], int now, int other) {
+    const int k0 = keys.lo + t * F::KT;
+    if (t + 2 < steps) fetch_k(t + 2);
+    fetch_v(t);
+    __syncthreads();
+    if (A.bits || k0 + F::KT > len) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) mask_scores(s[kb], k0 + 32 * kb, len, words, half);
+    }
+    float top = run.m;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+    top = other_max(top);
+    // the reference point only moves once a score passes it by 2^8 in the result: p then stays under 2^8, exact in every type, and the
+    // accumulators are rescaled a few times in all instead of once a tile
+    if (__any((top - run.m) * A.c > 8.f)) {  // (-inf against -inf: NaN, no)
+      add_values(vbuf + other);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) p[kb][0] = p[kb][1] = pack<T>(zero16(), 0);
+      const float to = top == -kInf ? 0.f : top * A.c;
+      const float alpha = __builtin_amdgcn_exp2f(run.m * A.c - to);  // (m = -inf: 0)
+      run.m = top;
+      run.l *= alpha;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] *= alpha;
+    }
+    const float base = run.base(A.c);
+    scores(kbuf + other, next);  // (behind the last tile: what lies in the buffer, not used)
+    add_values(vbuf + other);
+    // p is rounded to the tensor's type for the product (half a step relative to each p); its sum l keeps 32 bits
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], A.c, -base));
+        run.l += s[kb][i];
+      }
+      p[kb][0] = pack<T>(s[kb], 0);
+      p[kb][1] = pack<T>(s[kb], 1);
+    }
+    sk.store(kbuf + now);  // (no tile t + 2: what was there, not used)
+    sv.store(vbuf + now);
+  };
+  if (steps > 0) {
+    fetch_k(0);
+    sk.store(kbuf);
+    if (steps > 1) {
+      fetch_k(1);
+      sk.store(kbuf + F::TILE);
+    }
+    for (int i = threadIdx.x; i < F::TILE / 8; i += 256) reinterpret_cast<u32x4*>(vbuf + F::TILE)[i] = u32x4{0u, 0u, 0u, 0u};
+    __syncthreads();
+    f32x16 s0[KB], s1[KB];
+    scores(kbuf, s0);
+    for (int t = 0;; t += 2) {
+      step(t, s0, s1, 0, F::TILE);
+      if (t + 1 >= steps) break;
+      step(t + 1, s1, s0, F::TILE, 0);
+      if (t + 2 >= steps) break;
+    }
+    __syncthreads();
+    add_values(vbuf + ((steps - 1) & 1) * F::TILE);
+  }
+  const float l = both_sum(run.l);
+  if (r >= A.rows) return;
+  const Row row(A, hk, r);
+  const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const long long at = ((long long)b * A.Hk + hk) * A.rows + r;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int dd = 32 * d + reg_row(i, half);
+      if (dd >= A.D) continue;
+      if (A.splits > 1) {
+        float* o = A.part + (split * ((long long)A.B * A.Hk * A.rows) + at) * A.D + dd;
+        *reinterpret_cast<float4*>(o) = make_float4(acc[d][i] * f, acc[d][i + 1] * f, acc[d][i + 2] * f, acc[d][i + 3] * f);
+      } else {
+        typename Type<T>::x4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = (T)(acc[d][i + j] * f);
+        *reinterpret_cast<typename Type<T>::x4*>(static_cast<T*>(A.out) + row.packed(A, b) + dd) = y;
+      }
+    }
+  if (half == 0) {
+    const float lse = l > 0.f ? run.base(A.c) + log2f(l) : (l == 0.f ? -kInf : l);
     if (A.splits > 1) A.part_lse[split * ((long long)A.B * A.Hk * A.rows) + at] = lse;
     else if (A.lse) A.lse[at] = lse == -kInf ? kInf : lse;  // (+inf: the backward pass finds p = 0)
   }
@@ -382,14 +535,24 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const Args A) {
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------
 
-// dq: the forward's walk over the keys; two score-sized products and the one with K
+// dq: the walk over the keys again, p from the saved lse; per tile two score-sized products and the one with K.  The scores of tile t + 1 are
+// formed in the same basic block in which the vector unit turns those of tile t into ds, so there are three buffers (t, t + 1, and t + 2 filling).
+// RW = 4: a wave owns 32 rows; RW = 1 (at most 32 rows): the waves share the keys of a tile.
+template <int DP, int RW>
+struct Dq {
+  static constexpr int KW = 4 / RW, KB = RW == 4 && DP < 128 ? 2 : 1, KT = 32 * KB * KW, RT = 32 * RW, TILE = KT * Tile<DP>::PITCH;
+  static constexpr int BUFS = RW == 4 ? 3 : 1, LDS = 2 * BUFS * TILE * 2;
+  static_assert(KW == 1 || KW * 32 * DP * 4 <= 2 * TILE * 2, "the join of the waves fits the tiles");
+};
+
 template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(256) cross_dq_kernel(const Args A) {
-  typedef Fwd<T, DP, RW> F;
+__global__ void __launch_bounds__(256, 2) cross_dq_kernel(const Args A) {
+  typedef Dq<DP, RW> F;
   typedef typename Type<T>::x8 x8;
+  constexpr int KB = F::KB;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  T* Kt = reinterpret_cast<T*>(lds);
-  T* Vt = Kt + F::KT * DP;
+  T* kbuf = reinterpret_cast<T*>(lds);
+  T* vbuf = kbuf + F::BUFS * F::TILE;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int rw = wave % RW, kw = wave / RW;
   int id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -400,23 +563,24 @@ __global__ void __launch_bounds__(256) cross_dq_kernel(const Args A) {
   const int hk = id % A.Hk, b = id / A.Hk;
   const int r = tile * F::RT + rw * 32 + (lane & 31), len = length_of(A, b);
   const bool on = r < A.rows;
-  const Row row(A, hk, min(r, A.rows - 1));
   const Range keys = split_range(len, A.splits, split, F::KT);
-  const T* k = reinterpret_cast<const T*>(A.k) + b * A.kb + hk * A.kh;
-  const T* v = reinterpret_cast<const T*>(A.v) + b * A.vb + hk * A.vh;
-  const unsigned* words = A.bits ? A.bits + b * A.mb + row.h * A.mh + row.n * A.mn : nullptr;
+  const char* k = A.k + 2 * (b * A.kb + hk * A.kh);
+  const char* v = A.v + 2 * (b * A.vb + hk * A.vh);
   const unsigned* skip = A.bits && A.mn == 0 && (A.mh == 0 || A.G == 1) ? A.bits + b * A.mb + hk * A.mh : nullptr;
+  const unsigned* words = nullptr;
   const long long at = ((long long)b * A.Hk + hk) * A.rows + r;
   x8 q[DP / 16], g[DP / 16];
-  row_operand<T, DP>(reinterpret_cast<const T*>(A.q) + b * A.qb + row.n * A.qn + row.h * A.qh, A.D, on, q);
-  row_operand<T, DP>(static_cast<const T*>(A.dout) + row.packed(A, b), A.D, on, g);
   float delta = 0.f;
-  {  // do . o as the diagonal of a product: the same order of summation as do . v, so a row that sees one key has ds = 0 exactly
+  {
+    const Row row(A, hk, min(r, A.rows - 1));
+    const long long here = row.packed(A, b);
+    if (A.bits) words = A.bits + b * A.mb + row.h * A.mh + row.n * A.mn;
+    row_operand<T, DP>(reinterpret_cast<const T*>(A.q) + b * A.qb + row.n * A.qn + row.h * A.qh, A.D, on, q);
+    row_operand<T, DP>(static_cast<const T*>(A.dout) + here, A.D, on, g);
+    // do . o as the diagonal of a product: the same order of summation as do . v, so a row that sees one key has ds = 0 exactly
     x8 o[DP / 16];
-    row_operand<T, DP>(static_cast<const T*>(A.o) + row.packed(A, b), A.D, on, o);
-    f32x16 x;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    row_operand<T, DP>(static_cast<const T*>(A.o) + here, A.D, on, o);
+    f32x16 x = zero16();
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) x = Type<T>::mfma(o[d], g[d], x);
     const int c = lane & 31;
@@ -430,50 +594,115 @@ __global__ void __launch_bounds__(256) cross_dq_kernel(const Args A) {
   if (on && half == 0 && kw == 0 && split == 0) A.delta[at] = delta;
   f32x16 acc[DP / 32];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+  for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
   Stage<T, DP, F::KT> sk, sv;
-  for (int k0 = keys.lo; k0 < keys.hi; k0 += F::KT) {
-    sk.load(k, A.kn, k0, len, A.D, skip);
-    sv.load(v, A.vn, k0, len, A.D, skip);
+  sk.place(A.kn, A.D);
+  sv.place(A.vn, A.D);
+  const bool all = A.D == DP && !skip;
+  auto fetch = [&](int k0) {
+    const bool whole = all && k0 + F::KT <= len;
+    sk.load(k + 2 * k0 * A.kn, 2 * sk.STEP * A.kn, len - k0, whole, skip, k0);
+    sv.load(v + 2 * k0 * A.vn, 2 * sv.STEP * A.vn, len - k0, whole, skip, k0);
+  };
+  auto scores = [&](const T* Kt, f32x16 (&s)[KB]) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) s[kb] = Type<T>::mfma(operand<T, DP>(Kt, (kw * KB + kb) * 32, d), q[d], d ? s[kb] : zero16());
+  };
+  auto mask = [&](int k0, f32x16 (&s)[KB]) {
+    if (A.bits || k0 + F::KT > len) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) mask_scores(s[kb], k0 + (kw * KB + kb) * 32, len, words, half);
+    }
+  };
+  // ds, rounded to the tensor's type for the product (half a step relative to each).  States that no query sees were staged as zeros, so dp is
+  // finite where p is zero by a length or a shared mask.
+  auto gradient = [&](const T* Vt, const f32x16 (&s)[KB], x8 (&ds)[KB][2]) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      f32x16 dp;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) dp = Type<T>::mfma(operand<T, DP>(Vt, (kw * KB + kb) * 32, d), g[d], d ? dp : zero16());
+      f32x16 x;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], A.c, -lse));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= dp[i] - delta;
+      ds[kb][0] = pack<T>(x, 0);
+      ds[kb][1] = pack<T>(x, 1);
+    }
+  };
+  auto add_keys = [&](const T* Kt, const x8 (&ds)[KB][2]) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+          acc[d] = Type<T>::mfma(operand_t<T, DP>(Kt, (kw * KB + kb) * 32 + 16 * st, 32 * d), ds[kb][st], acc[d]);
+  };
+  const int steps = (keys.hi - keys.lo + F::KT - 1) / F::KT;
+  if (RW == 1) {
+    if (steps > 0) fetch(keys.lo);
+    for (int t = 0; t < steps; ++t) {
+      const int k0 = keys.lo + t * F::KT;
+      __syncthreads();
+      sk.store(kbuf);
+      sv.store(vbuf);
+      if (t + 1 < steps) fetch(k0 + F::KT);
+      __syncthreads();
+      f32x16 s[KB];
+      x8 ds[KB][2];
+      scores(kbuf, s);
+      mask(k0, s);
+      gradient(vbuf, s, ds);
+      add_keys(kbuf, ds);
+    }
+  } else if (steps > 0) {
+    fetch(keys.lo);
+    sk.store(kbuf);
+    sv.store(vbuf);
+    if (steps > 1) {
+      fetch(keys.lo + F::KT);
+      sk.store(kbuf + F::TILE);
+      sv.store(vbuf + F::TILE);
+    }
     __syncthreads();
-    sk.store(Kt);
-    sv.store(Vt);
-    __syncthreads();
-#pragma unroll
-    for (int kb = 0; kb < F::KB; ++kb) {
-      const int row0 = (kw * F::KB + kb) * 32;
-      f32x16 s, dp;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) s = Type<T>::mfma(operand<T, DP>(Kt, row0, d), q[d], s);
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) dp = Type<T>::mfma(operand<T, DP>(Vt, row0, d), g[d], dp);
-      mask_scores(s, k0 + row0, len, words, half);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[i], A.c, -lse));
-        s[i] = p == 0.f ? 0.f : p * (dp[i] - delta);  // (a blocked key's dp may be anything)
-      }
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const x8 ds = pack<T>(s, st);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mfma(operand_t<T, DP>(Kt, row0 + 16 * st, 32 * d), ds, acc[d]);
-      }
+    f32x16 s0[KB], s1[KB];
+    scores(kbuf, s0);
+    int kt = 0, kn = F::TILE, kf = 2 * F::TILE;  // K (and V) of tile t, t + 1, t + 2
+    auto step = [&](int t, f32x16 (&s)[KB], f32x16 (&next)[KB]) {
+      const int k0 = keys.lo + t * F::KT;
+      if (t + 2 < steps) fetch(k0 + 2 * F::KT);
+      __syncthreads();
+      mask(k0, s);
+      x8 ds[KB][2];
+      gradient(vbuf + kt, s, ds);
+      scores(kbuf + kn, next);  // (behind the last tile: what lies in the buffer, not used)
+      add_keys(kbuf + kt, ds);
+      sk.store(kbuf + kf);  // (no tile t + 2: what was there, not used)
+      sv.store(vbuf + kf);
+      const int x = kt;
+      kt = kn, kn = kf, kf = x;
+    };
+    for (int t = 0;; t += 2) {
+      step(t, s0, s1);
+      if (t + 1 >= steps) break;
+      step(t + 1, s1, s0);
+      if (t + 2 >= steps) break;
     }
   }
   auto store = [&](int d, const float (&x)[4]) {
     if (d >= A.D) return;
     if (A.splits > 1) {
-      float* o = A.part + ((((long long)split * A.B + b) * A.Hk + hk) * A.rows + r) * A.D + d;
+      float* o = A.part + (split * ((long long)A.B * A.Hk * A.rows) + at) * A.D + d;
       *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
     } else {
       typename Type<T>::x4 y;
 #pragma unroll
       for (int j = 0; j < 4; ++j) y[j] = (T)(x[j] * A.scale);
+      const Row row(A, hk, r);
       *reinterpret_cast<typename Type<T>::x4*>(static_cast<T*>(A.out) + row.packed(A, b) + d) = y;
     }
   };
@@ -531,20 +760,16 @@ __global__ void __launch_bounds__(256) cross_dq_sum_kernel(const Args A) {
 // the B operands of dV^T = dO^T P and dK^T = Q^T dS; lse and delta of a tile's rows lie in LDS.
 template <typename T, int DP>
 struct Bwd {
-  static constexpr int KT = 128, RT = 64 * 64 / DP < 32 ? 32 : (64 * 64 / DP > 64 ? 64 : 64 * 64 / DP);
-  static constexpr int LDS = 2 * RT * DP * 2 + 2 * RT * 4 + 4 * RT * 4;
+  static constexpr int KT = 128, RT = DP == 32 ? 64 : 32;
+  static constexpr int TILE = 2 * RT * Tile<DP>::PITCH * 2, SIDE = 2 * RT * 4 + 4 * RT * 4;  // Q and dO; lse, delta and the four waves' mask words
+  static constexpr int BUF = TILE + SIDE, LDS = 3 * BUF;
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) cross_dkv_kernel(const Args A) {
+__global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const Args A) {
   typedef Bwd<T, DP> F;
   typedef typename Type<T>::x8 x8;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  T* Qt = reinterpret_cast<T*>(lds);
-  T* Gt = Qt + F::RT * DP;
-  float* Lt = reinterpret_cast<float*>(Gt + F::RT * DP);
-  float* Dt = Lt + F::RT;
-  unsigned* Mt = reinterpret_cast<unsigned*>(Dt + F::RT);  // [4 waves][RT]: the mask words of the wave's keys
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   int id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int tile = id % A.tiles;
@@ -561,97 +786,166 @@ __global__ void __launch_bounds__(256) cross_dkv_kernel(const Args A) {
   row_operand<T, DP>(reinterpret_cast<const T*>(A.v) + b * A.vb + hk * A.vh + key * A.vn, A.D, open, v);
   f32x16 ak[DP / 32], av[DP / 32];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) ak[d][i] = av[d][i] = 0.f;
+  for (int d = 0; d < DP / 32; ++d) ak[d] = av[d] = zero16();
   const int row_tiles = (A.rows + F::RT - 1) / F::RT, per = (row_tiles + A.splits - 1) / A.splits;
   const int lo = split * per, hi = tile * F::KT < len ? min(row_tiles, (split + 1) * per) : lo;
   const T* q = reinterpret_cast<const T*>(A.q) + b * A.qb;
   const T* g = static_cast<const T*>(A.dout);
-  for (int rt = lo; rt < hi; ++rt) {
-    constexpr int N = F::RT * (DP / 8) / 256;
-    u32x4 rq[N], rg[N];
+  const long long side = ((long long)b * A.Hk + hk) * A.rows;
+  constexpr int N = F::RT * (DP / 8) / 256, STEP = 256 / (DP / 8);
+  // a thread's vectors of a tile; where G divides a tile's rows they move on by the same distance from tile to tile
+  const bool even = F::RT % A.G == 0 && A.D == DP;
+  const int c = threadIdx.x % (DP / 8), x0 = threadIdx.x / (DP / 8);
+  const int to = Tile<DP>::at(x0, c);
+  long long qat[N], gat[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int x = threadIdx.x + 256 * i, r = rt * F::RT + x / (DP / 8), c = x % (DP / 8);
-      u32x4 z = {0u, 0u, 0u, 0u};
-      rq[i] = rg[i] = z;
-      if (r < A.rows && c * 8 < A.D) {
-        const Row row(A, hk, r);
-        rq[i] = *reinterpret_cast<const u32x4*>(q + row.n * A.qn + row.h * A.qh + c * 8);
-        rg[i] = *reinterpret_cast<const u32x4*>(g + row.packed(A, b) + c * 8);
+  for (int i = 0; i < N; ++i) {
+    const Row row(A, hk, x0 + STEP * i);
+    qat[i] = row.n * A.qn + row.h * A.qh + c * 8;
+    gat[i] = row.packed(A, b) + c * 8;
+  }
+  const long long qstep = F::RT / A.G * A.qn, gstep = (long long)(F::RT / A.G) * A.Hq * A.D;
+  u32x4 rq[N], rg[N];
+  float rl = 0.f;
+  unsigned rm = 0u;
+  auto fetch = [&](int rt) {
+    if (even && (rt + 1) * F::RT <= A.rows) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        rq[i] = *reinterpret_cast<const u32x4*>(q + rt * qstep + qat[i]);
+        rg[i] = *reinterpret_cast<const u32x4*>(g + rt * gstep + gat[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = rt * F::RT + x0 + STEP * i;
+        rq[i] = rg[i] = u32x4{0u, 0u, 0u, 0u};
+        if (r < A.rows && c * 8 < A.D) {
+          const Row row(A, hk, r);
+          rq[i] = *reinterpret_cast<const u32x4*>(q + row.n * A.qn + row.h * A.qh + c * 8);
+          rg[i] = *reinterpret_cast<const u32x4*>(g + row.packed(A, b) + c * 8);
+        }
       }
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int x = threadIdx.x + 256 * i, at = Tile<DP>::at(x / (DP / 8), x % (DP / 8));
-      *reinterpret_cast<u32x4*>(Qt + at) = rq[i];
-      *reinterpret_cast<u32x4*>(Gt + at) = rg[i];
-    }
-    if (threadIdx.x < F::RT) {
-      const int r = rt * F::RT + threadIdx.x;
-      const long long at = ((long long)b * A.Hk + hk) * A.rows + r;
-      Lt[threadIdx.x] = r < A.rows ? A.lse[at] : kInf;
-      Dt[threadIdx.x] = r < A.rows ? A.delta[at] : 0.f;
+    if (threadIdx.x < 2 * F::RT) {  // the first RT threads: lse, the next: delta
+      const int r = rt * F::RT + threadIdx.x % F::RT;
+      const float* from = threadIdx.x < F::RT ? A.lse : A.delta;
+      rl = r < A.rows ? from[side + r] : (threadIdx.x < F::RT ? kInf : 0.f);
     }
     if (A.bits) {
-      for (int x = threadIdx.x; x < 4 * F::RT; x += 256) {
-        const int r = rt * F::RT + x % F::RT, w = tile * 4 + x / F::RT;
-        unsigned m = 0xffffffffu;
-        if (r < A.rows && w * 32 < A.Lk) {
-          const Row row(A, hk, r);
-          m = A.bits[b * A.mb + row.h * A.mh + row.n * A.mn + w];
-        }
-        Mt[x] = m;
+      const int x = threadIdx.x, r = rt * F::RT + x % F::RT, w = tile * 4 + x / F::RT;
+      rm = 0xffffffffu;
+      if (x < 4 * F::RT && r < A.rows && w * 32 < A.Lk) {
+        const Row row(A, hk, r);
+        rm = A.bits[b * A.mb + row.h * A.mh + row.n * A.mn + w];
       }
     }
-    __syncthreads();
-#pragma unroll 1
-    for (int rb = 0; rb < F::RT; rb += 32) {
-      f32x16 s, dp;
+  };
+  auto park = [&](char* buf) {
+    T* Qt = reinterpret_cast<T*>(buf);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+    for (int i = 0; i < N; ++i) {
+      *reinterpret_cast<u32x4*>(Qt + to + i * STEP * Tile<DP>::PITCH) = rq[i];
+      *reinterpret_cast<u32x4*>(Qt + (F::RT + i * STEP) * Tile<DP>::PITCH + to) = rg[i];
+    }
+    if (threadIdx.x < 2 * F::RT) reinterpret_cast<float*>(buf + F::TILE)[threadIdx.x] = rl;
+    if (A.bits && threadIdx.x < 4 * F::RT) reinterpret_cast<unsigned*>(buf + F::TILE + 2 * F::RT * 4)[threadIdx.x] = rm;
+  };
+  constexpr int RB = F::RT / 32;
+  auto scores = [&](const char* buf, f32x16 (&s)[RB]) {
+    const T* Qt = reinterpret_cast<const T*>(buf);
 #pragma unroll
-      for (int d = 0; d < DP / 16; ++d) s = Type<T>::mfma(operand<T, DP>(Qt, rb, d), k[d], s);
+    for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-      for (int d = 0; d < DP / 16; ++d) dp = Type<T>::mfma(operand<T, DP>(Gt, rb, d), v[d], dp);
+      for (int d = 0; d < DP / 16; ++d) s[rb] = Type<T>::mfma(operand<T, DP>(Qt, 32 * rb, d), k[d], d ? s[rb] : zero16());
+  };
+  auto mask = [&](const char* buf, f32x16 (&s)[RB]) {
+    if (!A.bits) return;
+    const unsigned* Mt = reinterpret_cast<const unsigned*>(buf + F::TILE + 2 * F::RT * 4) + wave * F::RT;
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const float4 L = *reinterpret_cast<const float4*>(Lt + rb + reg_row(i, half));
-        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], A.c, -L.x));
-        s[i + 1] = __builtin_amdgcn_exp2f(fmaf(s[i + 1], A.c, -L.y));
-        s[i + 2] = __builtin_amdgcn_exp2f(fmaf(s[i + 2], A.c, -L.z));
-        s[i + 3] = __builtin_amdgcn_exp2f(fmaf(s[i + 3], A.c, -L.w));
-      }
-      if (A.bits) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(Mt + wave * F::RT + rb + reg_row(i, half));
-          const unsigned bit = 1u << (lane & 31);
-          if (w.x & bit) s[i] = 0.f;
-          if (w.y & bit) s[i + 1] = 0.f;
-          if (w.z & bit) s[i + 2] = 0.f;
-          if (w.w & bit) s[i + 3] = 0.f;
-        }
-      }
+    for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
-        const float4 X = *reinterpret_cast<const float4*>(Dt + rb + reg_row(i, half));
-        dp[i] = s[i] == 0.f ? 0.f : s[i] * (dp[i] - X.x);
-        dp[i + 1] = s[i + 1] == 0.f ? 0.f : s[i + 1] * (dp[i + 1] - X.y);
-        dp[i + 2] = s[i + 2] == 0.f ? 0.f : s[i + 2] * (dp[i + 2] - X.z);
-        dp[i + 3] = s[i + 3] == 0.f ? 0.f : s[i + 3] * (dp[i + 3] - X.w);
-      }
+        const uint4 w = *reinterpret_cast<const uint4*>(Mt + 32 * rb + reg_row(i, half));
+        const unsigned w4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const x8 p = pack<T>(s, st), ds = pack<T>(dp, st);
+        for (int j = 0; j < 4; ++j)
+          if ((w4[j] >> (lane & 31)) & 1) s[rb][i + j] = -kInf;
+      }
+  };
+  // p and ds, rounded to the tensor's type for the products (half a step relative to each)
+  auto gradient = [&](const char* buf, const f32x16 (&s)[RB], x8 (&p)[RB][2], x8 (&ds)[RB][2]) {
+    const T* Gt = reinterpret_cast<const T*>(buf) + F::RT * Tile<DP>::PITCH;
+    const float* Lt = reinterpret_cast<const float*>(buf + F::TILE);
+    const float* Dt = Lt + F::RT;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      f32x16 dp;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) dp = Type<T>::mfma(operand<T, DP>(Gt, 32 * rb, d), v[d], d ? dp : zero16());
+      f32x16 x;
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const float4 L = *reinterpret_cast<const float4*>(Lt + 32 * rb + reg_row(i, half));
+        x[i] = __builtin_amdgcn_exp2f(fmaf(s[rb][i], A.c, -L.x));
+        x[i + 1] = __builtin_amdgcn_exp2f(fmaf(s[rb][i + 1], A.c, -L.y));
+        x[i + 2] = __builtin_amdgcn_exp2f(fmaf(s[rb][i + 2], A.c, -L.z));
+        x[i + 3] = __builtin_amdgcn_exp2f(fmaf(s[rb][i + 3], A.c, -L.w));
+      }
+      p[rb][0] = pack<T>(x, 0);
+      p[rb][1] = pack<T>(x, 1);
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const float4 X = *reinterpret_cast<const float4*>(Dt + 32 * rb + reg_row(i, half));
+        x[i] *= dp[i] - X.x;
+        x[i + 1] *= dp[i + 1] - X.y;
+        x[i + 2] *= dp[i + 2] - X.z;
+        x[i + 3] *= dp[i + 3] - X.w;
+      }
+      ds[rb][0] = pack<T>(x, 0);
+      ds[rb][1] = pack<T>(x, 1);
+    }
+  };
+  auto add_rows = [&](const char* buf, const x8 (&p)[RB][2], const x8 (&ds)[RB][2]) {
+    const T* Qt = reinterpret_cast<const T*>(buf);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
-          av[d] = Type<T>::mfma(operand_t<T, DP>(Gt, rb + 16 * st, 32 * d), p, av[d]);
-          ak[d] = Type<T>::mfma(operand_t<T, DP>(Qt, rb + 16 * st, 32 * d), ds, ak[d]);
+          av[d] = Type<T>::mfma(operand_t<T, DP>(Qt, F::RT + 32 * rb + 16 * st, 32 * d), p[rb][st], av[d]);
+          ak[d] = Type<T>::mfma(operand_t<T, DP>(Qt, 32 * rb + 16 * st, 32 * d), ds[rb][st], ak[d]);
         }
-      }
+  };
+  if (lo < hi) {
+    fetch(lo);
+    park(lds);
+    if (lo + 1 < hi) {
+      fetch(lo + 1);
+      park(lds + F::BUF);
+    }
+    __syncthreads();
+    f32x16 s0[RB], s1[RB];
+    scores(lds, s0);
+    int bt = 0, bn = F::BUF, bf = 2 * F::BUF;  // buffers of tile t, t + 1, t + 2
+    auto step = [&](int rt, f32x16 (&s)[RB], f32x16 (&next)[RB]) {
+      if (rt + 2 < hi) fetch(rt + 2);
+      __syncthreads();
+      mask(lds + bt, s);
+      x8 p[RB][2], ds[RB][2];
+      gradient(lds + bt, s, p, ds);
+      scores(lds + bn, next);  // (behind the last tile: what lies in the buffer, not used)
+      add_rows(lds + bt, p, ds);
+      park(lds + bf);
+      const int x = bt;
+      bt = bn, bn = bf, bf = x;
+    };
+    for (int rt = lo;; rt += 2) {
+      step(rt, s0, s1);
+      if (rt + 1 >= hi) break;
+      step(rt + 1, s1, s0);
+      if (rt + 2 >= hi) break;
     }
   }
   if (key >= A.Lk) return;
@@ -721,9 +1015,14 @@ __global__ void __launch_bounds__(256) cross_pack_kernel(const unsigned char* bl
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
+struct Walk {
+  int rows;              // of a workgroup: 32 (the waves share the keys of a tile), 128 or 256 (a wave has its own rows)
+  int tiles, splits;
+};
+
 struct Plan {
-  int narrow, tiles, splits;        // forward and dq
-  int key_tiles, row_splits;        // dk, dv
+  Walk fwd, dq;
+  int key_tiles, row_splits;  // dk, dv
 };
 
 int pick_splits(long long groups, int tiles) {
@@ -734,14 +1033,21 @@ int pick_splits(long long groups, int tiles) {
   return s < 1 ? 1 : (int)s;
 }
 
+Walk walk_of(long long rows, long long bh, int Lk, bool wide) {
+  Walk w;
+  w.rows = rows <= 32 ? 32 : 128;
+  w.tiles = (int)((rows + w.rows - 1) / w.rows);
+  const int kt = w.rows == 32 ? 128 : 64;
+  w.splits = pick_splits(bh * w.tiles, (Lk + kt - 1) / kt);
+  return w;
+}
+
 Plan plan_of(const combo_cross_attention_t& d) {
   Plan p;
   const int G = d.Hq / d.Hk;
   const long long rows = (long long)d.Lq * G, bh = (long long)d.B * d.Hk;
-  p.narrow = rows <= 32;
-  p.tiles = p.narrow ? 1 : (int)((rows + 127) / 128);
-  const int kt = p.narrow ? 128 : 64;
-  p.splits = pick_splits(bh * p.tiles, (d.Lk + kt - 1) / kt);
+  p.fwd = walk_of(rows, bh, d.Lk, true);
+  p.dq = walk_of(rows, bh, d.Lk, false);
   p.key_tiles = (d.Lk + 127) / 128;
   p.row_splits = pick_splits(bh * p.key_tiles, (int)((rows + 31) / 32));
   return p;
@@ -754,6 +1060,7 @@ bool desc_ok(const combo_cross_attention_t* d) {
   if (((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15) return false;
   for (int i = 0; i < 3; ++i)
     if ((d->q_stride[i] | d->k_stride[i] | d->v_stride[i]) & 7 || d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0) return false;
+  if (d->k_stride[1] > (1 << 22) || d->v_stride[1] > (1 << 22)) return false;  // (32-bit byte offsets inside a tile of 128 keys)
   const long long G = d->Hq / d->Hk;
   return (long long)d->Lq * G < (1ll << 30) && d->Lk < (1 << 30) && (long long)d->B * d->Hq * (((long long)d->Lq + 127) / 128 + ((long long)d->Lk + 127) / 128) < (1 << 24);
 }
@@ -790,10 +1097,11 @@ long long blocks_of(long long items) { return (items + 255) / 256; }
 
 template <typename T, int DP>
 int forward(Args& A, const Plan& p, hipStream_t st) {
-  A.tiles = p.tiles, A.splits = p.splits;
+  A.tiles = p.fwd.tiles, A.splits = p.fwd.splits;
   const long long grid = (long long)A.B * A.Hk * A.splits * A.tiles;
-  int rc = p.narrow ? launch<cross_forward_kernel<T, DP, 1>>(grid, Fwd<T, DP, 1>::LDS, A, st)
-                    : launch<cross_forward_kernel<T, DP, 4>>(grid, Fwd<T, DP, 4>::LDS, A, st);
+  int rc;
+  if (p.fwd.rows == 32) rc = launch<cross_few_kernel<T, DP>>(grid, Few<DP>::LDS, A, st);
+  else rc = launch<cross_wide_kernel<T, DP>>(grid, Wide<DP>::LDS, A, st);
   if (rc == 0 && A.splits > 1) rc = launch<cross_join_kernel<T>>(blocks_of((long long)A.B * A.Hk * A.rows * (A.D / 8)), 0, A, st);
   return rc;
 }
@@ -801,10 +1109,10 @@ int forward(Args& A, const Plan& p, hipStream_t st) {
 template <typename T, int DP>
 int backward(Args& A, const Plan& p, hipStream_t st) {
   float* part = A.part;
-  A.tiles = p.tiles, A.splits = p.splits;
+  A.tiles = p.dq.tiles, A.splits = p.dq.splits;
   const long long grid = (long long)A.B * A.Hk * A.splits * A.tiles;
-  int rc = p.narrow ? launch<cross_dq_kernel<T, DP, 1>>(grid, Fwd<T, DP, 1>::LDS, A, st)
-                    : launch<cross_dq_kernel<T, DP, 4>>(grid, Fwd<T, DP, 4>::LDS, A, st);
+  int rc = p.dq.rows == 32 ? launch<cross_dq_kernel<T, DP, 1>>(grid, Dq<DP, 1>::LDS, A, st)
+                           : launch<cross_dq_kernel<T, DP, 4>>(grid, Dq<DP, 4>::LDS, A, st);
   if (rc == 0 && A.splits > 1) rc = launch<cross_dq_sum_kernel<T>>(blocks_of((long long)A.B * A.Hk * A.rows * (A.D / 8)), 0, A, st);
   if (rc) return rc;
   if (!A.dk) return 0;
@@ -830,19 +1138,19 @@ long long combo_cross_attention_workspace(const combo_cross_attention_t* d, int 
   if (!desc_ok(d)) return -1;
   const Plan p = plan_of(*d);
   const long long rows = (long long)d->B * d->Hq * d->Lq;
-  const long long fwd = p.splits > 1 ? p.splits * rows * (d->D + (backward_pass ? 0 : 1)) : 0;
-  if (!backward_pass) return fwd * 4;
+  if (!backward_pass) return p.fwd.splits > 1 ? p.fwd.splits * rows * (d->D + 1) * 4 : 0;
+  const long long dq = p.dq.splits > 1 ? p.dq.splits * rows * d->D : 0;
   const long long dkv = p.row_splits > 1 ? 2ll * p.row_splits * d->B * d->Lk * d->Hk * d->D : 0;
-  return ((fwd > dkv ? fwd : dkv) + rows) * 4;
+  return ((dq > dkv ? dq : dkv) + rows) * 4;
 }
 
 int combo_cross_attention_forward(const combo_cross_attention_t* d, void* out, float* lse, void* workspace, combo_stream_t stream) {
   if (!desc_ok(d) || !out || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 31)) return COMBO_EINVAL;
   const Plan p = plan_of(*d);
-  if (p.splits > 1 && !workspace) return COMBO_EINVAL;
+  if (p.fwd.splits > 1 && !workspace) return COMBO_EINVAL;
   Args A = args_of(*d);
   A.out = out, A.lse = lse, A.part = static_cast<float*>(workspace);
-  if (p.splits > 1) A.part_lse = A.part + (long long)p.splits * d->B * d->Hq * d->Lq * d->D;
+  if (p.fwd.splits > 1) A.part_lse = A.part + (long long)p.fwd.splits * d->B * d->Hq * d->Lq * d->D;
   return d->dtype == 1 ? by_dim<__bf16>(A, p, false, (hipStream_t)stream) : by_dim<_Float16>(A, p, false, (hipStream_t)stream);
 }
 

@@ -18,8 +18,10 @@ def _strides(t):
 
 
 def _readable(t):
-    """t as the kernels read it - whole 16-byte vectors of a contiguous last dimension -, copied only where it is not laid out so"""
-    if t.stride(3) == 1 and not any(s % 8 for s in _strides(t)) and t.data_ptr() % 16 == 0:
+    """t as the kernels read it - whole 16-byte vectors of a contiguous last dimension, tokens at most 2^22 elements apart -, copied only where it
+    is not laid out so"""
+    b, n, h = _strides(t)
+    if t.stride(3) == 1 and not (b | n | h) % 8 and n <= 1 << 22 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

@@ -669,7 +669,7 @@ int combo_adamw_f32(float* param, const float* grad, float* exp_avg, float* exp_
  *   clear; a row without an open key gives zeros and passes no gradient.  States behind a sample's length, and states blocked by a mask
  *   that all queries share (bits_stride[2] == 0 and the heads of a group share it), are never part of a product, whatever they hold.
  *   q [B,Lq,Hq,D], k / v [B,Lk,Hk,D]: strides (batch, token, head) in elements, multiples of 8, the last dimension contiguous, pointers
- *   16-byte aligned.  Hk divides Hq, D % 8 == 0, D <= 128, scale > 0.  dtype 1 bf16, 2 fp16.
+ *   16-byte aligned; tokens of k and v at most 2^22 elements apart.  Hk divides Hq, D % 8 == 0, D <= 128, scale > 0.  dtype 1 bf16, 2 fp16.
  *   kv_lengths [B] (nullable; clamped to 0 .. Lk).  blocked_bits (nullable): word w of a line holds the keys 32 w .. 32 w + 31, 1 = blocked;
  *   bits_stride: (batch, query head, query) in words, 0 where shared; combo_cross_attention_pack writes it from a byte (bool) mask
  *   [B,H,N,Lk] with strides in bytes into [B,H,N,(Lk+31)/32].
