@@ -669,28 +669,22 @@ __global__ void __launch_bounds__(256, 2) cross_dq_kernel(const Args A) {
       sv.store(vbuf + F::TILE);
     }
     __syncthreads();
-    f32x16 s0[KB], s1[KB];
-    scores(kbuf, s0);
+    f32x16 s[KB];
+    scores(kbuf, s);
     int kt = 0, kn = F::TILE, kf = 2 * F::TILE;  // K (and V) of tile t, t + 1, t + 2
-    auto step = [&](int t, f32x16 (&s)[KB], f32x16 (&next)[KB]) {
+    for (int t = 0; t < steps; ++t) {
       const int k0 = keys.lo + t * F::KT;
       if (t + 2 < steps) fetch(k0 + 2 * F::KT);
       __syncthreads();
       mask(k0, s);
       x8 ds[KB][2];
       gradient(vbuf + kt, s, ds);
-      scores(kbuf + kn, next);  // (behind the last tile: what lies in the buffer, not used)
+      scores(kbuf + kn, s);  // (behind the last tile: what lies in the buffer, not used)
       add_keys(kbuf + kt, ds);
       sk.store(kbuf + kf);  // (no tile t + 2: what was there, not used)
       sv.store(vbuf + kf);
       const int x = kt;
       kt = kn, kn = kf, kf = x;
-    };
-    for (int t = 0;; t += 2) {
-      step(t, s0, s1);
-      if (t + 1 >= steps) break;
-      step(t + 1, s1, s0);
-      if (t + 2 >= steps) break;
     }
   }
   auto store = [&](int d, const float (&x)[4]) {
@@ -852,13 +846,6 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
     if (A.bits && threadIdx.x < 4 * F::RT) reinterpret_cast<unsigned*>(buf + F::TILE + 2 * F::RT * 4)[threadIdx.x] = rm;
   };
   constexpr int RB = F::RT / 32;
-  auto scores = [&](const char* buf, f32x16 (&s)[RB]) {
-    const T* Qt = reinterpret_cast<const T*>(buf);
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) s[rb] = Type<T>::mfma(operand<T, DP>(Qt, 32 * rb, d), k[d], d ? s[rb] : zero16());
-  };
   auto mask = [&](const char* buf, f32x16 (&s)[RB]) {
     if (!A.bits) return;
     const unsigned* Mt = reinterpret_cast<const unsigned*>(buf + F::TILE + 2 * F::RT * 4) + wave * F::RT;
@@ -873,51 +860,57 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
           if ((w4[j] >> (lane & 31)) & 1) s[rb][i + j] = -kInf;
       }
   };
-  // p and ds, rounded to the tensor's type for the products (half a step relative to each)
-  auto gradient = [&](const char* buf, const f32x16 (&s)[RB], x8 (&p)[RB][2], x8 (&ds)[RB][2]) {
-    const T* Gt = reinterpret_cast<const T*>(buf) + F::RT * Tile<DP>::PITCH;
-    const float* Lt = reinterpret_cast<const float*>(buf + F::TILE);
-    const float* Dt = Lt + F::RT;
+  // The compiler places an LDS read right before the instruction that needs it, and with one or two waves on a SIMD its latency then shows at every
+  // product.  So a tile is worked in four stages that nothing is moved across; a stage's products take operands that the stage before has read,
+  // and its vector instructions do not wait for its own products:
+  //     dP of tile t               | p = exp2(S)               | reads Q of tile t + 1
+  //     S of tile t + 1            | ds = p (dP - delta)       | reads dO^T of tile t
+  //     dV += dO^T p               |                           | reads Q^T of tile t
+  //     dK += Q^T ds               |                           | reads dO and lse of tile t + 1
+  constexpr int ND = DP / 16, NT = DP / 32;
+  typedef x8 Rows[RB][ND];      // operands of a product over the head dimension
+  typedef x8 Cols[RB][2][NT];   // operands of a product over the tile's rows
+  auto read_rows = [&](const T* Xt, Rows& x) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      f32x16 dp;
+    for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-      for (int d = 0; d < DP / 16; ++d) dp = Type<T>::mfma(operand<T, DP>(Gt, 32 * rb, d), v[d], d ? dp : zero16());
-      f32x16 x;
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const float4 L = *reinterpret_cast<const float4*>(Lt + 32 * rb + reg_row(i, half));
-        x[i] = __builtin_amdgcn_exp2f(fmaf(s[rb][i], A.c, -L.x));
-        x[i + 1] = __builtin_amdgcn_exp2f(fmaf(s[rb][i + 1], A.c, -L.y));
-        x[i + 2] = __builtin_amdgcn_exp2f(fmaf(s[rb][i + 2], A.c, -L.z));
-        x[i + 3] = __builtin_amdgcn_exp2f(fmaf(s[rb][i + 3], A.c, -L.w));
-      }
-      p[rb][0] = pack<T>(x, 0);
-      p[rb][1] = pack<T>(x, 1);
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const float4 X = *reinterpret_cast<const float4*>(Dt + 32 * rb + reg_row(i, half));
-        x[i] *= dp[i] - X.x;
-        x[i + 1] *= dp[i + 1] - X.y;
-        x[i + 2] *= dp[i + 2] - X.z;
-        x[i + 3] *= dp[i + 3] - X.w;
-      }
-      ds[rb][0] = pack<T>(x, 0);
-      ds[rb][1] = pack<T>(x, 1);
-    }
+      for (int d = 0; d < ND; ++d) x[rb][d] = operand<T, DP>(Xt, 32 * rb, d);
   };
-  auto add_rows = [&](const char* buf, const x8 (&p)[RB][2], const x8 (&ds)[RB][2]) {
-    const T* Qt = reinterpret_cast<const T*>(buf);
+  auto read_cols = [&](const T* Xt, Cols& x) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          av[d] = Type<T>::mfma(operand_t<T, DP>(Qt, F::RT + 32 * rb + 16 * st, 32 * d), p[rb][st], av[d]);
-          ak[d] = Type<T>::mfma(operand_t<T, DP>(Qt, 32 * rb + 16 * st, 32 * d), ds[rb][st], ak[d]);
-        }
+        for (int d = 0; d < NT; ++d) x[rb][st][d] = operand_t<T, DP>(Xt, 32 * rb + 16 * st, 32 * d);
   };
+  auto q_tile = [&](int buf) { return reinterpret_cast<const T*>(lds + buf); };
+  auto g_tile = [&](int buf) { return reinterpret_cast<const T*>(lds + buf) + F::RT * Tile<DP>::PITCH; };
+  auto over_rows = [&](const Rows& x, const x8 (&y)[ND], f32x16 (&o)[RB]) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[rb] = Type<T>::mfma(x[rb][d], y[d], d ? o[rb] : zero16());
+  };
+  auto over_cols = [&](const Cols& x, const x8 (&y)[RB][2], f32x16 (&o)[NT]) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int d = 0; d < NT; ++d) o[d] = Type<T>::mfma(x[rb][st][d], y[rb][st], o[d]);
+  };
+  // a value per row (lse or delta) for this lane's 16 rows of each block
+  auto read_side = [&](const float* side_, f32x16 (&x)[RB]) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(side_ + 32 * rb + reg_row(i, half));
+        x[rb][i] = y.x, x[rb][i + 1] = y.y, x[rb][i + 2] = y.z, x[rb][i + 3] = y.w;
+      }
+  };
+  auto lse_of = [&](int buf) { return reinterpret_cast<const float*>(lds + buf + F::TILE); };
   if (lo < hi) {
     fetch(lo);
     park(lds);
@@ -926,26 +919,51 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
       park(lds + F::BUF);
     }
     __syncthreads();
-    f32x16 s0[RB], s1[RB];
-    scores(lds, s0);
+    f32x16 s[RB], dp[RB], x[RB], L[RB];
+    Rows rows;
+    Cols cols, cols2;
+    read_rows(q_tile(0), rows);
+    over_rows(rows, k, s);
+    read_rows(g_tile(0), rows);
+    read_side(lse_of(0), L);
     int bt = 0, bn = F::BUF, bf = 2 * F::BUF;  // buffers of tile t, t + 1, t + 2
-    auto step = [&](int rt, f32x16 (&s)[RB], f32x16 (&next)[RB]) {
+    for (int rt = lo; rt < hi; ++rt) {
       if (rt + 2 < hi) fetch(rt + 2);
       __syncthreads();
       mask(lds + bt, s);
+      over_rows(rows, v, dp);
+      Rows next;
+      read_rows(q_tile(bn), next);  // (behind the last tile: what lies in the buffer, not used)
       x8 p[RB][2], ds[RB][2];
-      gradient(lds + bt, s, p, ds);
-      scores(lds + bn, next);  // (behind the last tile: what lies in the buffer, not used)
-      add_rows(lds + bt, p, ds);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[rb][i] = __builtin_amdgcn_exp2f(fmaf(s[rb][i], A.c, -L[rb][i]));
+        // p, and ds below, are rounded to the tensor's type for the products (half a step relative to each)
+        p[rb][0] = pack<T>(x[rb], 0);
+        p[rb][1] = pack<T>(x[rb], 1);
+      }
+      read_side(lse_of(bt) + F::RT, L);  // delta
+      __builtin_amdgcn_sched_barrier(0);
+      over_rows(next, k, s);
+      read_cols(g_tile(bt), cols);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[rb][i] *= dp[rb][i] - L[rb][i];
+        ds[rb][0] = pack<T>(x[rb], 0);
+        ds[rb][1] = pack<T>(x[rb], 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      over_cols(cols, p, av);
+      read_cols(q_tile(bt), cols2);
+      __builtin_amdgcn_sched_barrier(0);
+      over_cols(cols2, ds, ak);
+      read_rows(g_tile(bn), rows);
+      read_side(lse_of(bn), L);
       park(lds + bf);
-      const int x = bt;
-      bt = bn, bn = bf, bf = x;
-    };
-    for (int rt = lo;; rt += 2) {
-      step(rt, s0, s1);
-      if (rt + 1 >= hi) break;
-      step(rt + 1, s1, s0);
-      if (rt + 2 >= hi) break;
+      const int y = bt;
+      bt = bn, bn = bf, bf = y;
     }
   }
   if (key >= A.Lk) return;
