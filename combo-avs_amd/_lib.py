@@ -5,6 +5,9 @@ this package falls back to PyTorch/CPU for an op that has a HIP kernel.
 """
 import ctypes
 import os
+import weakref
+
+import torch as _torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libcombo_avs_hip.so")
@@ -182,12 +185,12 @@ def check(code, what):
         raise HipError(f"{what} failed with hipError_t {code}")
 
 
-def _float_types():
-    import torch
-    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+FLOAT_TYPES = {_torch.float32: 0, _torch.bfloat16: 1, _torch.float16: 2}  # dtype codes of the entry points that take several types
 
-
-FLOAT_TYPES = _float_types()  # dtype codes of the entry points that take several types
+# the current device and a device's current stream as plain integers: torch.cuda.current_stream() builds a Stream object, 4 us of a
+# small launch's 14 (a torch built without GPU support has neither function; nothing is launched there)
+_current_device = getattr(_torch._C, "_cuda_getDevice", None) or (lambda: _torch.cuda.current_device())
+_raw_stream = getattr(_torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: _torch.cuda.current_stream(index).cuda_stream)
 
 
 def ptr(t):
@@ -202,41 +205,41 @@ def current_stream():
 
 
 
-_LEAF_MARK = "combo_avs_default_stream"
+_eager_graphs = weakref.WeakKeyDictionary()  # {autograd node recorded on the default stream: its leaves (weak)}
 
 
 def record(function, *args):
     """function.apply(*args).  Autograd keeps ONE accumulation node per leaf, alive as long as any graph of the leaf, and that node remembers
     the stream on which it was made.  If that is the default stream, a backward pass that is captured into a graph has to join it,
-    which ends the process when the capture does: so an eager call on the default stream marks the nodes of its leaves, and a call inside a
-    capture that finds a marked node alive refuses."""
+    which ends the process when the capture does: so a call inside a capture refuses while a graph of one of its leaves that an eager call on the
+    default stream has recorded is alive."""
     import torch
     if torch.cuda.is_current_stream_capturing():
-        for t in args:
-            if torch.is_tensor(t) and t.requires_grad and t.is_leaf and _LEAF_MARK in torch.autograd.graph.get_gradient_edge(t).node.metadata:
-                raise RuntimeError("a graph is being captured while an eager autograd graph of the same leaf, recorded on the default stream, is "
-                                   "alive: drop its outputs (or detach them) before the capture, or record them on another stream")
+        leaves = [t for t in args if torch.is_tensor(t) and t.requires_grad and t.is_leaf]
+        if any(ref() is t for refs in list(_eager_graphs.values()) for ref in refs for t in leaves):
+            raise RuntimeError("a graph is being captured while an eager autograd graph of the same leaf, recorded on the default stream, is "
+                               "alive: drop its outputs (or detach them) before the capture, or record them on another stream")
         return function.apply(*args)
     out = function.apply(*args)
-    if current_stream() == 0:
-        for node, _ in out.grad_fn.next_functions:
-            if type(node).__name__ == "AccumulateGrad":
-                node.metadata[_LEAF_MARK] = True
+    if _raw_stream(_current_device()) == 0:
+        leaves = [weakref.ref(t) for t in args if torch.is_tensor(t) and t.requires_grad and t.is_leaf]
+        if leaves:
+            _eager_graphs[out.grad_fn] = leaves
     return out
 
 
 class device_of:
     """`with device_of(t) as stream:` t's device is current inside the block; stream: that device's current stream"""
+    __slots__ = ("index", "guard")
 
     def __init__(self, t):
-        self.index, self.guard = t.device.index, None
+        self.index, self.guard = t.get_device(), None
 
     def __enter__(self):
-        import torch
-        if self.index is not None and self.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.index)
+        if self.index != _current_device():
+            self.guard = _torch.cuda.device(self.index)
             self.guard.__enter__()
-        return current_stream()
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.guard is not None:

@@ -24,21 +24,45 @@ enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec { T v[V]; };
 
+// 1 / x to one unit in the last place (v_rcp_f32): a full division is ten instructions, and an activation map is short of them - SiLU by
+// division took 39 us for a 64 MB bf16 map, half of it in the vector unit
+__device__ __forceinline__ float quick_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ float sigmoid(float z) { return quick_rcp(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z)); }
+// the normal distribution function by erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x) (Abramowitz and Stegun 7.1.26, error under 1.5e-7):
+// the small side keeps its relative size, and the exponential is the one of the density below
+__device__ __forceinline__ float normal_cdf(float z, float& density) {
+  const float x = fabsf(z) * 0.70710678f, t = quick_rcp(fmaf(0.3275911f, x, 1.f)), e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+  float q = fmaf(t, 1.061405429f, -1.453152027f);
+  q = fmaf(t, q, 1.421413741f);
+  q = fmaf(t, q, -0.284496736f);
+  q = fmaf(t, q, 0.254829592f);
+  const float tail = 0.5f * q * t * e;
+  density = 0.39894228f * e;
+  return z < 0.f ? tail : 1.f - tail;
+}
+
 template <int ACT>
 __device__ __forceinline__ float act(float z) {
   if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;  // (a NaN stays one)
-  if constexpr (ACT == ACT_SILU) return z / (1.f + __expf(-z));
-  if constexpr (ACT == ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  if constexpr (ACT == ACT_SILU) return z * sigmoid(z);
+  if constexpr (ACT == ACT_GELU) {
+    float d;
+    return z * normal_cdf(z, d);
+  }
   return z;
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (ACT == ACT_SILU) {
-    const float s = 1.f / (1.f + __expf(-z));
-    return s * (1.f + z * (1.f - s));
+    const float s = sigmoid(z);
+    return s * fmaf(z, 1.f - s, 1.f);
   }
-  if constexpr (ACT == ACT_GELU) return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+  if constexpr (ACT == ACT_GELU) {
+    float d;
+    const float c = normal_cdf(z, d);
+    return fmaf(z, d, c);
+  }
   return 1.f;
 }
 
@@ -101,9 +125,10 @@ __device__ __forceinline__ void join_stats(int entries, int team, int lane, F ge
   M2 = team_sum(q, team);
 }
 
-// per-channel (mean, M2) of a token range into LDS: stat[rows][range][2]
+// (mean, M2) of a token range into LDS: stat[rows][range / step][2], an entry for `step` neighbouring channels - V where a group is made of whole
+// vectors, else 1
 template <typename T, int V>
-__device__ __forceinline__ void channel_stats(const T* x, int C, int range, int t0, int t1, const Lanes& L, float* stat) {
+__device__ __forceinline__ void channel_stats(const T* x, int C, int range, int step, int t0, int t1, const Lanes& L, float* stat) {
   if (!L.on) return;
   for (int ch = L.chunk; ch * V < range; ch += kThreads) {
     const T* p = x + (long long)(t0 + L.row) * C + ch * V;
@@ -116,39 +141,70 @@ __device__ __forceinline__ void channel_stats(const T* x, int C, int range, int 
 #pragma unroll
       for (int k = 0; k < V; ++k) K[k] = (float)a.v[k];
       n = (t1 - t0 - L.row + L.rows - 1) / L.rows;
-      const long long step = (long long)L.rows * C;
+      const long long next = (long long)L.rows * C;
 #pragma unroll 4
       for (int i = 1; i < n; ++i) {
-        p += step;
+        p += next;
         const Vec<T, V> b = *reinterpret_cast<const Vec<T, V>*>(p);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           const float d = (float)b.v[k] - K[k];
           s[k] += d;
-          q[k] += d * d;
+          q[k] = fmaf(d, d, q[k]);
         }
       }
     }
     const float inv = n > 0 ? 1.f / (float)n : 0.f;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      float* o = stat + (L.row * range + ch * V + k) * 2;
-      o[0] = K[k] + s[k] * inv;
-      o[1] = q[k] - s[k] * s[k] * inv;
+      q[k] -= s[k] * s[k] * inv;
+      K[k] += s[k] * inv;
+    }
+    float* o = stat + (L.row * range + ch * V) / step * 2;
+    if (step == 1) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        o[2 * k] = K[k];
+        o[2 * k + 1] = q[k];
+      }
+    } else {
+      float m = 0.f, M2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < V; ++k) m += K[k];
+      m *= 1.f / V;
+#pragma unroll
+      for (int k = 0; k < V; ++k) M2 += fmaf((K[k] - m) * (K[k] - m), (float)n, q[k]);
+      o[0] = m;
+      o[1] = M2;
     }
   }
 }
 
-__device__ __forceinline__ void group_of_stat(const float* stat, int range, int per, int rows, int tokens, int g, int team, int lane, float& n,
-                                              float& mean, float& M2) {
-  join_stats(rows * per, team, lane,
-             [&](int i, float& ni, float& mi, float& qi) {
-               const int r = i / per, c = g * per + (i - r * per);
-               ni = r < tokens ? (float)((tokens - r + rows - 1) / rows) : 0.f;
-               mi = stat[(r * range + c) * 2];
-               qi = stat[(r * range + c) * 2 + 1];
-             },
-             n, mean, M2);
+// group g's statistics out of stat: a lane takes rows
+__device__ __forceinline__ void group_of_stat(const float* stat, int range, int per, int step, int rows, int tokens, int g, int team, int lane,
+                                              float& n, float& mean, float& M2) {
+  const int width = range / step, q = per / step;
+  const float* p = stat + 2 * g * q;
+  float sn = 0.f, sm = 0.f;
+  for (int r = lane; r < rows; r += team) {
+    const float ni = r < tokens ? (float)((tokens - r + rows - 1) / rows) * step : 0.f;
+    float m = 0.f;
+    for (int c = 0; c < q; ++c) m += p[(r * width + c) * 2];
+    sn += ni * q;
+    sm += ni * m;
+  }
+  n = team_sum(sn, team);
+  mean = n > 0.f ? team_sum(sm, team) / n : 0.f;
+  float s2 = 0.f;
+  for (int r = lane; r < rows; r += team) {
+    if (r >= tokens) continue;
+    const float ni = (float)((tokens - r + rows - 1) / rows) * step;
+    for (int c = 0; c < q; ++c) {
+      const float d = p[(r * width + c) * 2] - mean;
+      s2 += fmaf(ni * d, d, p[(r * width + c) * 2 + 1]);
+    }
+  }
+  M2 = team_sum(s2, team);
 }
 
 // partial statistics of one slice
@@ -158,13 +214,14 @@ __global__ void __launch_bounds__(kThreads) gna_stats_kernel(const NormArgs A) {
   const int b = blockIdx.x / A.S, s = blockIdx.x - b * A.S;
   const int t0 = s * A.slice, t1 = min(A.HW, t0 + A.slice);
   const Lanes L(A.C / V);
-  channel_stats<T, V>(static_cast<const T*>(A.x) + (long long)b * A.HW * A.C, A.C, A.C, t0, t1, L, sh);
+  const int step = A.per % V == 0 ? V : 1;
+  channel_stats<T, V>(static_cast<const T*>(A.x) + (long long)b * A.HW * A.C, A.C, A.C, step, t0, t1, L, sh);
   __syncthreads();
   const int team = team_size(A.G), lane = threadIdx.x & (team - 1);
   for (int g0 = 0; g0 < A.G; g0 += kThreads / team) {
     const int g = g0 + threadIdx.x / team;
     float n, mean, M2;
-    group_of_stat(sh, A.C, A.per, L.rows, t1 - t0, min(g, A.G - 1), team, lane, n, mean, M2);
+    group_of_stat(sh, A.C, A.per, step, L.rows, t1 - t0, min(g, A.G - 1), team, lane, n, mean, M2);
     if (lane == 0 && g < A.G) {
       float* o = A.part + (((long long)b * A.S + s) * A.G + g) * 2;
       o[0] = mean;
@@ -195,7 +252,7 @@ __device__ __forceinline__ void apply_tokens(const NormArgs& A, int b, int c0, i
       const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + off);
       Vec<T, V> o;
 #pragma unroll
-      for (int k = 0; k < V; ++k) o.v[k] = (T)act<ACT>(((float)v.v[k] - m[k]) * a[k] + bb[k]);
+      for (int k = 0; k < V; ++k) o.v[k] = (T)act<ACT>(fmaf((float)v.v[k] - m[k], a[k], bb[k]));
       *reinterpret_cast<Vec<T, V>*>(y + off) = o;
     }
   }
@@ -224,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) gna_apply_kernel(const NormArgs A, i
       const float r = rstd_of(M2, n, A.eps);
       sh[g] = mean;
       sh[A.G + g] = r;
-      if (s == 0) {
+      if (s == 0 && A.mean) {
         A.mean[b * A.G + g] = mean;
         A.rstd[b * A.G + g] = r;
       }
@@ -242,20 +299,23 @@ __global__ void __launch_bounds__(kThreads) gna_forward_kernel(const NormArgs A)
   const int parts = A.C / A.range, b = blockIdx.x / parts, c0 = (blockIdx.x - b * parts) * A.range;
   const int gn = A.range / A.per, g00 = c0 / A.per;
   const Lanes L(A.range / V);
-  channel_stats<T, V>(static_cast<const T*>(A.x) + (long long)b * A.HW * A.C + c0, A.C, A.range, 0, A.HW, L, sh);
+  const int step = A.per % V == 0 ? V : 1;
+  channel_stats<T, V>(static_cast<const T*>(A.x) + (long long)b * A.HW * A.C + c0, A.C, A.range, step, 0, A.HW, L, sh);
   __syncthreads();
   float* mr = sh + (size_t)L.rows * A.range * 2;
   const int team = team_size(gn), lane = threadIdx.x & (team - 1);
   for (int g0 = 0; g0 < gn; g0 += kThreads / team) {
     const int g = min(g0 + (int)threadIdx.x / team, gn - 1);
     float n, mean, M2;
-    group_of_stat(sh, A.range, A.per, L.rows, A.HW, g, team, lane, n, mean, M2);
+    group_of_stat(sh, A.range, A.per, step, L.rows, A.HW, g, team, lane, n, mean, M2);
     if (lane == 0) {
       const float r = rstd_of(M2, n, A.eps);
       mr[g] = mean;
       mr[gn + g] = r;
-      A.mean[b * A.G + g00 + g] = mean;
-      A.rstd[b * A.G + g00 + g] = r;
+      if (A.mean) {
+        A.mean[b * A.G + g00 + g] = mean;
+        A.rstd[b * A.G + g00 + g] = r;
+      }
     }
   }
   __syncthreads();
@@ -289,9 +349,9 @@ __device__ __forceinline__ void channel_grads(const NormArgs& A, int b, int c0, 
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const float xh = ((float)xv.v[k] - m[k]) * r[k];
-        const float dz = (float)gv.v[k] * act_slope<ACT>(xh * w[k] + bb[k]);
+        const float dz = (float)gv.v[k] * act_slope<ACT>(fmaf(xh, w[k], bb[k]));
         u[k] += dz;
-        v[k] += dz * xh;
+        v[k] = fmaf(dz, xh, v[k]);
       }
     }
 #pragma unroll
@@ -365,8 +425,8 @@ __device__ __forceinline__ void dx_tokens(const NormArgs& A, int b, int c0, int 
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const float xh = ((float)xv.v[k] - m[k]) * r[k];
-        const float dz = (float)gv.v[k] * act_slope<ACT>(xh * w[k] + bb[k]);
-        o.v[k] = (T)(r[k] * (dz * w[k] - a1[k] - xh * a2[k]));
+        const float dz = (float)gv.v[k] * act_slope<ACT>(fmaf(xh, w[k], bb[k]));
+        o.v[k] = (T)(r[k] * fmaf(-xh, a2[k], fmaf(dz, w[k], -a1[k])));
       }
       *reinterpret_cast<Vec<T, V>*>(dx + off) = o;
     }
@@ -485,10 +545,11 @@ size_t lds_floats(int range, int V) {
   return (size_t)rows * range * 2;
 }
 
-// slices of an image: >= 1024 workgroups over the batch where the map is large, at least 16 tokens and 16 KiB in each
+// slices of an image: the batch makes just under 1024 workgroups, four for each CU (40 images in 26 slices were 1040, and the CUs with five
+// of them finished last: 39 us against 31), with at least 16 tokens and 8 KiB in each
 void choose_slices(NormArgs& A, int size) {
-  long long by_bytes = ((long long)A.HW * A.C * size + 16383) / 16384;
-  long long want = (1024 + A.B - 1) / A.B;
+  long long by_bytes = ((long long)A.HW * A.C * size + 8191) / 8192;
+  long long want = 1024 / A.B;
   long long S = by_bytes < want ? by_bytes : want;
   if (S > (A.HW + 15) / 16) S = (A.HW + 15) / 16;
   if (S > 256) S = 256;
@@ -567,7 +628,8 @@ extern "C" {
 long long combo_groupnorm_act_workspace(int B, int HW, int C, int G, int dtype, int backward_pass) {
   if (!shape_ok(B, HW, C, G, dtype, 0)) return -1;
   NormArgs A = {};
-  A.B = B, A.HW = HW, A.C = C, A.G = G;
+  A.B = B, A.HW = HW, A.C = C, A.G = G, A.range = C;
+  if (!backward_pass && one_launch(A, dtype == 0 ? 4 : 2)) return 0;
   choose_slices(A, dtype == 0 ? 4 : 2);
   const long long rows = (long long)B * A.S;
   return rows * G * 2 + (backward_pass ? rows * C * 2 : 0);
@@ -575,7 +637,8 @@ long long combo_groupnorm_act_workspace(int B, int HW, int C, int G, int dtype, 
 
 int combo_groupnorm_act_forward(const void* x, const float* weight, const float* bias, int B, int HW, int C, int G, float eps, int act_,
                                 int dtype, float* workspace, float* mean, float* rstd, void* y, combo_stream_t stream) {
-  if (!x || !workspace || !mean || !rstd || !y || !shape_ok(B, HW, C, G, dtype, act_)) return COMBO_EINVAL;
+  if (!x || (!mean) != (!rstd) || !y || !shape_ok(B, HW, C, G, dtype, act_)) return COMBO_EINVAL;
+  if (!workspace && combo_groupnorm_act_workspace(B, HW, C, G, dtype, 0) > 0) return COMBO_EINVAL;
   const uintptr_t all = (uintptr_t)x | (uintptr_t)y;
   if (all & (dtype == 0 ? 3 : 1)) return COMBO_EINVAL;
   NormArgs A = {};

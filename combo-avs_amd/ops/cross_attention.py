@@ -14,7 +14,9 @@ _DESC = struct.Struct("3Q9q2Q3q7if")  # combo_cross_attention_t
 
 
 def _strides(t):
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
+    a, b, c, _ = t.stride()
+    l, m, n, _ = t.shape
+    return a if l > 1 else 0, b if m > 1 else 0, c if n > 1 else 0
 
 
 def _readable(t):

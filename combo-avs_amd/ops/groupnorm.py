@@ -65,22 +65,23 @@ def _channels_last(x):
     return torch.channels_last if x.dim() == 4 else torch.channels_last_3d
 
 
-def _act_workspace(x, groups, code, backward):
-    n = _lib.lib().combo_groupnorm_act_workspace(x.shape[0], x.shape[2:].numel(), x.shape[1], groups, code, 1 if backward else 0)
-    return torch.empty(n, device=x.device, dtype=torch.float32)
+def _act_workspace(x, places, groups, code, backward):
+    n = _lib.lib().combo_groupnorm_act_workspace(x.shape[0], places, x.shape[1], groups, code, backward)
+    return torch.empty(n, device=x.device, dtype=torch.float32) if n else None
 
 
-def _act_forward(x, weight, bias, groups, eps, act):
-    B, C = x.shape[:2]
+def _act_forward(x, weight, bias, groups, eps, act, keep=False):
+    """-> (y, mean and rstd [2, B, groups] for the backward pass or None)"""
+    B, C, places = x.shape[0], x.shape[1], x.shape[2:].numel()
     y = torch.empty_like(x)  # (preserves channels_last)
-    stats = torch.empty(2, B, groups, device=x.device, dtype=torch.float32)
+    stats = torch.empty(2, B, groups, device=x.device, dtype=torch.float32) if keep else None
     if x.numel() == 0:
         return y, stats
-    code, base = _lib.FLOAT_TYPES[x.dtype], stats.data_ptr()
+    code, mean = _lib.FLOAT_TYPES[x.dtype], _lib.ptr(stats)
     with _lib.device_of(x) as stream:
-        ws = _act_workspace(x, groups, code, False)
-        _lib.check(_lib.lib().combo_groupnorm_act_forward(x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), B, x.shape[2:].numel(), C, groups,
-                                                          eps, act, code, ws.data_ptr(), base, base + 4 * B * groups, y.data_ptr(), stream),
+        ws = _act_workspace(x, places, groups, code, 0)
+        _lib.check(_lib.lib().combo_groupnorm_act_forward(x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), B, places, C, groups, eps, act, code,
+                                                          _lib.ptr(ws), mean, mean + 4 * B * groups if keep else 0, y.data_ptr(), stream),
                    "combo_groupnorm_act_forward")
     return y, stats
 
@@ -88,7 +89,7 @@ def _act_forward(x, weight, bias, groups, eps, act):
 class _GroupNormAct(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        y, stats = _act_forward(x, weight, bias, groups, eps, act)
+        y, stats = _act_forward(x, weight, bias, groups, eps, act, True)
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.groups, ctx.act = groups, act
         return y
@@ -105,11 +106,11 @@ class _GroupNormAct(Function):
         if x.numel() == 0:
             return dx, dw, db, None, None, None
         dy = dy.contiguous(memory_format=_channels_last(x))
-        code, base = _lib.FLOAT_TYPES[x.dtype], stats.data_ptr()
+        code, base, places = _lib.FLOAT_TYPES[x.dtype], stats.data_ptr(), x.shape[2:].numel()
         with _lib.device_of(x) as stream:
-            ws = _act_workspace(x, ctx.groups, code, True)
+            ws = _act_workspace(x, places, ctx.groups, code, 1)
             _lib.check(_lib.lib().combo_groupnorm_act_backward(dy.data_ptr(), x.data_ptr(), _lib.ptr(weight), _lib.ptr(bias), base,
-                                                               base + 4 * B * ctx.groups, B, x.shape[2:].numel(), C, ctx.groups, ctx.act, code,
+                                                               base + 4 * B * ctx.groups, B, places, C, ctx.groups, ctx.act, code,
                                                                ws.data_ptr(), dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), stream),
                        "combo_groupnorm_act_backward")
         return dx, dw, db, None, None, None

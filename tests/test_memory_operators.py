@@ -48,7 +48,10 @@ def test_entry_points_refuse_bad_arguments_without_a_launch():
     assert all(rc == 1 for rc in (rotary(D=7), rotary(D=2), rotary(D=258), rotary(axes=0), rotary(axes=9), rotary(pos_type=4), rotary(dtype=3),
                                   rotary(B=0), rotary(x=0), rotary(x=4098), rotary(H=1 << 25)))
     assert lib.combo_groupnorm_act_workspace(1, 9, 8, 3, 0, 0) == -1 and lib.combo_groupnorm_act_workspace(1, 9, 4104, 2, 0, 0) == -1
-    assert lib.combo_groupnorm_act_workspace(2, 9, 8, 2, 0, 0) == 8 and lib.combo_groupnorm_act_workspace(2, 9, 8, 2, 0, 1) == 40
+    assert lib.combo_groupnorm_act_workspace(2, 9, 8, 2, 0, 0) == 0 and lib.combo_groupnorm_act_workspace(2, 9, 8, 2, 0, 1) == 40
+    assert lib.combo_groupnorm_act_workspace(2, 9000, 64, 2, 0, 0) > 0
+    assert lib.combo_groupnorm_act_forward(one, 0, 0, 2, 9000, 64, 2, 1e-5, 0, 0, 0, one, one, one, 0) == 1  # two launches need their workspace
+    assert lib.combo_groupnorm_act_forward(one, 0, 0, 1, 9, 8, 2, 1e-5, 0, 0, 0, one, 0, one, 0) == 1  # mean without rstd
     assert lib.combo_groupnorm_act_forward(one, 0, 0, 1, 9, 8, 3, 1e-5, 0, 0, one, one, one, one, 0) == 1
     assert lib.combo_groupnorm_act_forward(one, 0, 0, 1, 9, 8, 2, 1e-5, 4, 0, one, one, one, one, 0) == 1
     assert lib.combo_groupnorm_act_forward(one + 2, 0, 0, 1, 9, 8, 2, 1e-5, 0, 0, one, one, one, one, 0) == 1
