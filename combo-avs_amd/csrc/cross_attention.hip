@@ -171,20 +171,31 @@ __device__ __forceinline__ void row_operand(const T* p, int D, bool on, typename
   }
 }
 
-// scores of keys key0 .. key0 + 31 against this lane's row: lengths and mask
-__device__ __forceinline__ void mask_scores(f32x16& s, int key0, int len, const unsigned* words, int half) {
+// scores of keys key0 .. key0 + 31 against this lane's row: length and mask word
+__device__ __forceinline__ void mask_scores(f32x16& s, int key0, int len, bool masked, unsigned word, int half) {
   if (key0 + 32 > len) {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if (key0 + reg_row(i, half) >= len) s[i] = -kInf;
   }
-  if (words) {
-    const unsigned w = (key0 < len ? words[key0 >> 5] : 0xffffffffu) >> (4 * half);
+  if (masked) {
+    const unsigned w = word >> (4 * half);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if (w & (1u << (8 * (i >> 2) + (i & 3)))) s[i] = -kInf;
   }
 }
+
+// a row's mask words of one tile (N blocks of 32 keys from key0 on), read a tile ahead of their use
+template <int N>
+struct Words {
+  unsigned w[N];
+  __device__ __forceinline__ void load(const unsigned* words, int key0, int len) {
+    if (!words) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = key0 + 32 * i < len ? words[(key0 >> 5) + i] : 0xffffffffu;
+  }
+};
 
 struct Range { int lo, hi; };
 // the keys of split `s`: whole tiles of the sample's own length
@@ -249,17 +260,25 @@ __global__ void __launch_bounds__(256, 2) cross_few_kernel(const Args A) {
     sk.load(k + 2 * k0 * A.kn, 2 * sk.STEP * A.kn, len - k0, whole, skip, k0);
     sv.load(v + 2 * k0 * A.vn, 2 * sv.STEP * A.vn, len - k0, whole, skip, k0);
   };
-  if (keys.lo < keys.hi) fetch(keys.lo);
+  Words<1> now = {}, ahead = {};
+  if (keys.lo < keys.hi) {
+    fetch(keys.lo);
+    ahead.load(words, keys.lo + 32 * kw, len);
+  }
   for (int k0 = keys.lo; k0 < keys.hi; k0 += F::KT) {
     __syncthreads();
     sk.store(Kt);
     sv.store(Vt);
-    if (k0 + F::KT < keys.hi) fetch(k0 + F::KT);  // the next tile travels while this one is multiplied
+    now = ahead;
+    if (k0 + F::KT < keys.hi) {  // the next tile travels while this one is multiplied
+      fetch(k0 + F::KT);
+      ahead.load(words, k0 + F::KT + 32 * kw, len);
+    }
     __syncthreads();
     f32x16 s;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) s = Type<T>::mfma(operand<T, DP>(Kt, 32 * kw, d), q[d], d ? s : zero16());
-    if (A.bits || k0 + F::KT > len) mask_scores(s, k0 + 32 * kw, len, words, half);
+    if (A.bits || k0 + F::KT > len) mask_scores(s, k0 + 32 * kw, len, A.bits, now.w[0], half);
     float top = run.m;
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
@@ -384,9 +403,9 @@ __global__ void __launch_bounds__(256, 2) cross_wide_kernel(const Args A) {
   sv.place(A.vn, A.D);
   const bool all = A.D == DP && !skip;
   const int steps = (keys.hi - keys.lo + F::KT - 1) / F::KT;
-  auto fetch_k = [&](int t) {
+  auto fetch_k = [&](Stage<T, DP, F::KT>& to, int t) {
     const int k0 = keys.lo + t * F::KT;
-    sk.load(k + 2 * k0 * A.kn, 2 * sk.STEP * A.kn, len - k0, all && k0 + F::KT <= len, skip, k0);
+    to.load(k + 2 * k0 * A.kn, 2 * sk.STEP * A.kn, len - k0, all && k0 + F::KT <= len, skip, k0);
   };
   auto fetch_v = [&](int t) {
     const int k0 = keys.lo + t * F::KT;
@@ -411,14 +430,16 @@ __global__ void __launch_bounds__(256, 2) cross_wide_kernel(const Args A) {
   };
   Running run;
   // tile t: its scores s; the scores of tile t + 1 go to `next`; `now`, `other`: the buffers of tile t and of its neighbours
+  Words<KB> mask = {};
   auto step = [&](int t, f32x16 (&s)[KB], f32x16 (&next)[KB], int now, int other) {
     const int k0 = keys.lo + t * F::KT;
-    if (t + 2 < steps) fetch_k(t + 2);
+    if (t + 2 < steps) fetch_k(sk, t + 2);
     fetch_v(t);
     __syncthreads();
     if (A.bits || k0 + F::KT > len) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) mask_scores(s[kb], k0 + 32 * kb, len, words, half);
+      for (int kb = 0; kb < KB; ++kb) mask_scores(s[kb], k0 + 32 * kb, len, A.bits, mask.w[kb], half);
+      mask.load(words, k0 + F::KT, len);
     }
     float top = run.m;
 #pragma unroll
@@ -459,12 +480,12 @@ __global__ void __launch_bounds__(256, 2) cross_wide_kernel(const Args A) {
     sv.store(vbuf + now);
   };
   if (steps > 0) {
-    fetch_k(0);
+    Stage<T, DP, F::KT> k1 = sk;
+    fetch_k(sk, 0);
+    if (steps > 1) fetch_k(k1, 1);
+    mask.load(words, keys.lo, len);
     sk.store(kbuf);
-    if (steps > 1) {
-      fetch_k(1);
-      sk.store(kbuf + F::TILE);
-    }
+    if (steps > 1) k1.store(kbuf + F::TILE);
     for (int i = threadIdx.x; i < F::TILE / 8; i += 256) reinterpret_cast<u32x4*>(vbuf + F::TILE)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
     f32x16 s0[KB], s1[KB];
@@ -546,7 +567,7 @@ struct Dq {
 };
 
 template <typename T, int DP, int RW>
-__global__ void __launch_bounds__(256, 2) cross_dq_kernel(const Args A) {
+__global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_kernel(const Args A) {
   typedef Dq<DP, RW> F;
   typedef typename Type<T>::x8 x8;
   constexpr int KB = F::KB;
@@ -569,6 +590,20 @@ __global__ void __launch_bounds__(256, 2) cross_dq_kernel(const Args A) {
   const unsigned* skip = A.bits && A.mn == 0 && (A.mh == 0 || A.G == 1) ? A.bits + b * A.mb + hk * A.mh : nullptr;
   const unsigned* words = nullptr;
   const long long at = ((long long)b * A.Hk + hk) * A.rows + r;
+  Stage<T, DP, F::KT> sk, sv;
+  sk.place(A.kn, A.D);
+  sv.place(A.vn, A.D);
+  const bool all = A.D == DP && !skip;
+  auto fetch = [&](Stage<T, DP, F::KT>& sk, Stage<T, DP, F::KT>& sv, int k0) {
+    const bool whole = all && k0 + F::KT <= len;
+    sk.load(k + 2 * k0 * A.kn, 2 * sk.STEP * A.kn, len - k0, whole, skip, k0);
+    sv.load(v + 2 * k0 * A.vn, 2 * sv.STEP * A.vn, len - k0, whole, skip, k0);
+  };
+  const int steps = (keys.hi - keys.lo + F::KT - 1) / F::KT;
+  // the first tiles travel together with the rows
+  Stage<T, DP, F::KT> k1 = sk, v1 = sv;
+  if (steps > 0) fetch(sk, sv, keys.lo);
+  if (RW == 4 && steps > 1) fetch(k1, v1, keys.lo + F::KT);
   x8 q[DP / 16], g[DP / 16];
   float delta = 0.f;
   {
@@ -595,25 +630,18 @@ __global__ void __launch_bounds__(256, 2) cross_dq_kernel(const Args A) {
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
-  Stage<T, DP, F::KT> sk, sv;
-  sk.place(A.kn, A.D);
-  sv.place(A.vn, A.D);
-  const bool all = A.D == DP && !skip;
-  auto fetch = [&](int k0) {
-    const bool whole = all && k0 + F::KT <= len;
-    sk.load(k + 2 * k0 * A.kn, 2 * sk.STEP * A.kn, len - k0, whole, skip, k0);
-    sv.load(v + 2 * k0 * A.vn, 2 * sv.STEP * A.vn, len - k0, whole, skip, k0);
-  };
   auto scores = [&](const T* Kt, f32x16 (&s)[KB]) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) s[kb] = Type<T>::mfma(operand<T, DP>(Kt, (kw * KB + kb) * 32, d), q[d], d ? s[kb] : zero16());
   };
+  Words<KB> bits = {};
   auto mask = [&](int k0, f32x16 (&s)[KB]) {
     if (A.bits || k0 + F::KT > len) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) mask_scores(s[kb], k0 + (kw * KB + kb) * 32, len, words, half);
+      for (int kb = 0; kb < KB; ++kb) mask_scores(s[kb], k0 + (kw * KB + kb) * 32, len, A.bits, bits.w[kb], half);
+      bits.load(words, k0 + F::KT + kw * KB * 32, len);
     }
   };
   // ds, rounded to the tensor's type for the product (half a step relative to each).  States that no query sees were staged as zeros, so dp is
@@ -642,15 +670,14 @@ __global__ void __launch_bounds__(256, 2) cross_dq_kernel(const Args A) {
         for (int d = 0; d < DP / 32; ++d)
           acc[d] = Type<T>::mfma(operand_t<T, DP>(Kt, (kw * KB + kb) * 32 + 16 * st, 32 * d), ds[kb][st], acc[d]);
   };
-  const int steps = (keys.hi - keys.lo + F::KT - 1) / F::KT;
+  bits.load(words, keys.lo + kw * KB * 32, len);
   if (RW == 1) {
-    if (steps > 0) fetch(keys.lo);
     for (int t = 0; t < steps; ++t) {
       const int k0 = keys.lo + t * F::KT;
       __syncthreads();
       sk.store(kbuf);
       sv.store(vbuf);
-      if (t + 1 < steps) fetch(k0 + F::KT);
+      if (t + 1 < steps) fetch(sk, sv, k0 + F::KT);
       __syncthreads();
       f32x16 s[KB];
       x8 ds[KB][2];
@@ -660,13 +687,11 @@ __global__ void __launch_bounds__(256, 2) cross_dq_kernel(const Args A) {
       add_keys(kbuf, ds);
     }
   } else if (steps > 0) {
-    fetch(keys.lo);
     sk.store(kbuf);
     sv.store(vbuf);
     if (steps > 1) {
-      fetch(keys.lo + F::KT);
-      sk.store(kbuf + F::TILE);
-      sv.store(vbuf + F::TILE);
+      k1.store(kbuf + F::TILE);
+      v1.store(vbuf + F::TILE);
     }
     __syncthreads();
     f32x16 s[KB];
@@ -674,14 +699,14 @@ __global__ void __launch_bounds__(256, 2) cross_dq_kernel(const Args A) {
     int kt = 0, kn = F::TILE, kf = 2 * F::TILE;  // K (and V) of tile t, t + 1, t + 2
     for (int t = 0; t < steps; ++t) {
       const int k0 = keys.lo + t * F::KT;
-      if (t + 2 < steps) fetch(k0 + 2 * F::KT);
+      if (t + 2 < steps) fetch(sk, sv, k0 + 2 * F::KT);
       __syncthreads();
       mask(k0, s);
       x8 ds[KB][2];
       gradient(vbuf + kt, s, ds);
       scores(kbuf + kn, s);  // (behind the last tile: what lies in the buffer, not used)
       add_keys(kbuf + kt, ds);
-      sk.store(kbuf + kf);  // (no tile t + 2: what was there, not used)
+      sk.store(kbuf + kf);  // tile t + 2 (none left: what was there, not used)
       sv.store(vbuf + kf);
       const int x = kt;
       kt = kn, kn = kf, kf = x;
@@ -1043,9 +1068,10 @@ struct Plan {
   int key_tiles, row_splits;  // dk, dv
 };
 
+// Workgroups over the other axis when there are few: two for each of the 256 CUs, at least one tile each.  From one workgroup a CU on, a short axis
+// is left whole: 320 workgroups of 13 tiles take 26.8 us, and in two halves 22.7 us and a join of 4.2 us and one more launch.
 int pick_splits(long long groups, int tiles) {
-  // two workgroups for each of the 256 CUs; a split has at least one tile
-  long long s = (512 + groups - 1) / groups;
+  long long s = groups >= 256 && tiles < 32 ? 1 : (512 + groups - 1) / groups;
   if (s > tiles) s = tiles;
   if (s > 128) s = 128;
   return s < 1 ? 1 : (int)s;
