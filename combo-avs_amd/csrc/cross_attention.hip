@@ -171,6 +171,22 @@ __device__ __forceinline__ void row_operand(const T* p, int D, bool on, typename
   }
 }
 
+// 32 dimensions (d0 ..) of this lane's row, times f: the two halves of a wave hold alternate quads of a row, so each hands the other one of every two
+// and both write 16 bytes
+template <typename T>
+__device__ __forceinline__ void put_row(T* row, const f32x16& x, float f, int d0, int D, int half) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    typename Type<T>::x4 a, b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = (T)(x[i + j] * f), b[j] = (T)(x[i + 4 + j] * f);
+    const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
+    const auto lo = __builtin_amdgcn_permlane32_swap(ua.x, ub.x, false, false), hi = __builtin_amdgcn_permlane32_swap(ua.y, ub.y, false, false);
+    const int d = d0 + 2 * i + 8 * half;
+    if (d < D) *reinterpret_cast<u32x4*>(row + d) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+  }
+}
+
 // scores of keys key0 .. key0 + 31 against this lane's row: length and mask word
 __device__ __forceinline__ void mask_scores(f32x16& s, int key0, int len, bool masked, unsigned word, int half) {
   if (key0 + 32 > len) {
@@ -504,22 +520,20 @@ __global__ void __launch_bounds__(256, 2) cross_wide_kernel(const Args A) {
   const Row row(A, hk, r);
   const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   const long long at = ((long long)b * A.Hk + hk) * A.rows + r;
+  if (A.splits > 1) {
+    float* o = A.part + (split * ((long long)A.B * A.Hk * A.rows) + at) * A.D;
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int dd = 32 * d + reg_row(i, half);
-      if (dd >= A.D) continue;
-      if (A.splits > 1) {
-        float* o = A.part + (split * ((long long)A.B * A.Hk * A.rows) + at) * A.D + dd;
-        *reinterpret_cast<float4*>(o) = make_float4(acc[d][i] * f, acc[d][i + 1] * f, acc[d][i + 2] * f, acc[d][i + 3] * f);
-      } else {
-        typename Type<T>::x4 y;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = (T)(acc[d][i + j] * f);
-        *reinterpret_cast<typename Type<T>::x4*>(static_cast<T*>(A.out) + row.packed(A, b) + dd) = y;
+      for (int i = 0; i < 16; i += 4) {
+        const int dd = 32 * d + reg_row(i, half);
+        if (dd < A.D) *reinterpret_cast<float4*>(o + dd) = make_float4(acc[d][i] * f, acc[d][i + 1] * f, acc[d][i + 2] * f, acc[d][i + 3] * f);
       }
-    }
+  } else {
+    T* o = static_cast<T*>(A.out) + row.packed(A, b);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) put_row(o, acc[d], f, 32 * d, A.D, half);
+  }
   if (half == 0) {
     const float lse = l > 0.f ? run.base(A.c) + log2f(l) : (l == 0.f ? -kInf : l);
     if (A.splits > 1) A.part_lse[split * ((long long)A.B * A.Hk * A.rows) + at] = lse;
@@ -555,6 +569,21 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const Args A) {
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------
+
+// o . do of this lane's row as the diagonal of a product: the same order of summation as do . v, so a row that sees one key has ds = 0 exactly
+template <typename T, int DP>
+__device__ __forceinline__ float row_dot(const typename Type<T>::x8 (&o)[DP / 16], const typename Type<T>::x8 (&g)[DP / 16]) {
+  f32x16 x = zero16();
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) x = Type<T>::mfma(o[d], g[d], x);
+  const int c = threadIdx.x & 31;
+  float delta = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (4 * (c >> 3) + (c & 3) == i) delta = x[i];
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(delta), __float_as_uint(delta), false, false);
+  return __uint_as_float((c >> 2) & 1 ? sw[1] : sw[0]);
+}
 
 // dq: the walk over the keys again, p from the saved lse; per tile two score-sized products and the one with K.  The scores of tile t + 1 are
 // formed in the same basic block in which the vector unit turns those of tile t into ds, so there are three buffers (t, t + 1, and t + 2 filling).
@@ -612,18 +641,9 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
     if (A.bits) words = A.bits + b * A.mb + row.h * A.mh + row.n * A.mn;
     row_operand<T, DP>(reinterpret_cast<const T*>(A.q) + b * A.qb + row.n * A.qn + row.h * A.qh, A.D, on, q);
     row_operand<T, DP>(static_cast<const T*>(A.dout) + here, A.D, on, g);
-    // do . o as the diagonal of a product: the same order of summation as do . v, so a row that sees one key has ds = 0 exactly
     x8 o[DP / 16];
     row_operand<T, DP>(static_cast<const T*>(A.o) + here, A.D, on, o);
-    f32x16 x = zero16();
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) x = Type<T>::mfma(o[d], g[d], x);
-    const int c = lane & 31;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (4 * (c >> 3) + (c & 3) == i) delta = x[i];
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(delta), __float_as_uint(delta), false, false);
-    delta = __uint_as_float((c >> 2) & 1 ? sw[1] : sw[0]);
+    delta = row_dot<T, DP>(o, g);
   }
   const float lse = on ? A.lse[at] : kInf;
   if (on && half == 0 && kw == 0 && split == 0) A.delta[at] = delta;
@@ -748,13 +768,19 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
     }
   } else {
     if (!on) return;
+    if (A.splits > 1) {
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+      for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const float x[4] = {acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
-        store(32 * d + reg_row(i, half), x);
-      }
+        for (int i = 0; i < 16; i += 4) {
+          const float x[4] = {acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+          store(32 * d + reg_row(i, half), x);
+        }
+    } else {
+      T* o = static_cast<T*>(A.out) + Row(A, hk, r).packed(A, b);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) put_row(o, acc[d], A.scale, 32 * d, A.D, half);
+    }
   }
 }
 
@@ -992,32 +1018,29 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
     }
   }
   if (key >= A.Lk) return;
-  const bool mine = open;  // (keys behind the length or blocked for all: zeros)
+  if (!open) {  // keys behind the length or blocked for all: zeros
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) ak[d] = av[d] = zero16();
+  }
   const long long at = (((long long)b * A.Lk + key) * A.Hk + hk) * A.D, all = (long long)A.B * A.Lk * A.Hk * A.D;
+  if (A.splits > 1) {
+    float* o = A.part + 2 * split * all + at;
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int dd = 32 * d + reg_row(i, half);
-      if (dd >= A.D) continue;
-      float x[4], y[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] = mine ? ak[d][i + j] * A.scale : 0.f;
-        y[j] = mine ? av[d][i + j] : 0.f;
+      for (int i = 0; i < 16; i += 4) {
+        const int dd = 32 * d + reg_row(i, half);
+        if (dd >= A.D) continue;
+        *reinterpret_cast<float4*>(o + dd) = make_float4(ak[d][i] * A.scale, ak[d][i + 1] * A.scale, ak[d][i + 2] * A.scale, ak[d][i + 3] * A.scale);
+        *reinterpret_cast<float4*>(o + all + dd) = make_float4(av[d][i], av[d][i + 1], av[d][i + 2], av[d][i + 3]);
       }
-      if (A.splits > 1) {
-        float* o = A.part + 2 * split * all + at + dd;
-        *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4*>(o + all) = make_float4(y[0], y[1], y[2], y[3]);
-      } else {
-        typename Type<T>::x4 a, c;
+  } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = (T)x[j], c[j] = (T)y[j];
-        *reinterpret_cast<typename Type<T>::x4*>(static_cast<T*>(A.dk) + at + dd) = a;
-        *reinterpret_cast<typename Type<T>::x4*>(static_cast<T*>(A.dv) + at + dd) = c;
-      }
+    for (int d = 0; d < DP / 32; ++d) {
+      put_row(static_cast<T*>(A.dk) + at, ak[d], A.scale, 32 * d, A.D, half);
+      put_row(static_cast<T*>(A.dv) + at, av[d], 1.f, 32 * d, A.D, half);
     }
+  }
 }
 
 // sums the splits of dk and dv: 8 values a thread
@@ -1058,13 +1081,9 @@ __global__ void __launch_bounds__(256) cross_pack_kernel(const unsigned char* bl
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
-struct Walk {
-  int rows;              // of a workgroup: 32 (the waves share the keys of a tile), 128 or 256 (a wave has its own rows)
-  int tiles, splits;
-};
-
 struct Plan {
-  Walk fwd, dq;
+  int rows;                   // forward and dq: of a workgroup, 32 (the waves share the keys of a tile) or 128 (a wave has its own)
+  int tiles, splits;
   int key_tiles, row_splits;  // dk, dv
 };
 
@@ -1077,21 +1096,14 @@ int pick_splits(long long groups, int tiles) {
   return s < 1 ? 1 : (int)s;
 }
 
-Walk walk_of(long long rows, long long bh, int Lk, bool wide) {
-  Walk w;
-  w.rows = rows <= 32 ? 32 : 128;
-  w.tiles = (int)((rows + w.rows - 1) / w.rows);
-  const int kt = w.rows == 32 ? 128 : 64;
-  w.splits = pick_splits(bh * w.tiles, (Lk + kt - 1) / kt);
-  return w;
-}
-
 Plan plan_of(const combo_cross_attention_t& d) {
   Plan p;
   const int G = d.Hq / d.Hk;
   const long long rows = (long long)d.Lq * G, bh = (long long)d.B * d.Hk;
-  p.fwd = walk_of(rows, bh, d.Lk, true);
-  p.dq = walk_of(rows, bh, d.Lk, false);
+  p.rows = rows <= 32 ? 32 : 128;
+  p.tiles = (int)((rows + p.rows - 1) / p.rows);
+  const int kt = p.rows == 32 ? 128 : 64;
+  p.splits = pick_splits(bh * p.tiles, (d.Lk + kt - 1) / kt);
   p.key_tiles = (d.Lk + 127) / 128;
   p.row_splits = pick_splits(bh * p.key_tiles, (int)((rows + 31) / 32));
   return p;
@@ -1141,11 +1153,9 @@ long long blocks_of(long long items) { return (items + 255) / 256; }
 
 template <typename T, int DP>
 int forward(Args& A, const Plan& p, hipStream_t st) {
-  A.tiles = p.fwd.tiles, A.splits = p.fwd.splits;
+  A.tiles = p.tiles, A.splits = p.splits;
   const long long grid = (long long)A.B * A.Hk * A.splits * A.tiles;
-  int rc;
-  if (p.fwd.rows == 32) rc = launch<cross_few_kernel<T, DP>>(grid, Few<DP>::LDS, A, st);
-  else rc = launch<cross_wide_kernel<T, DP>>(grid, Wide<DP>::LDS, A, st);
+  int rc = p.rows == 32 ? launch<cross_few_kernel<T, DP>>(grid, Few<DP>::LDS, A, st) : launch<cross_wide_kernel<T, DP>>(grid, Wide<DP>::LDS, A, st);
   if (rc == 0 && A.splits > 1) rc = launch<cross_join_kernel<T>>(blocks_of((long long)A.B * A.Hk * A.rows * (A.D / 8)), 0, A, st);
   return rc;
 }
@@ -1153,10 +1163,9 @@ int forward(Args& A, const Plan& p, hipStream_t st) {
 template <typename T, int DP>
 int backward(Args& A, const Plan& p, hipStream_t st) {
   float* part = A.part;
-  A.tiles = p.dq.tiles, A.splits = p.dq.splits;
+  A.tiles = p.tiles, A.splits = p.splits;
   const long long grid = (long long)A.B * A.Hk * A.splits * A.tiles;
-  int rc = p.dq.rows == 32 ? launch<cross_dq_kernel<T, DP, 1>>(grid, Dq<DP, 1>::LDS, A, st)
-                           : launch<cross_dq_kernel<T, DP, 4>>(grid, Dq<DP, 4>::LDS, A, st);
+  int rc = p.rows == 32 ? launch<cross_dq_kernel<T, DP, 1>>(grid, Dq<DP, 1>::LDS, A, st) : launch<cross_dq_kernel<T, DP, 4>>(grid, Dq<DP, 4>::LDS, A, st);
   if (rc == 0 && A.splits > 1) rc = launch<cross_dq_sum_kernel<T>>(blocks_of((long long)A.B * A.Hk * A.rows * (A.D / 8)), 0, A, st);
   if (rc) return rc;
   if (!A.dk) return 0;
@@ -1182,8 +1191,8 @@ long long combo_cross_attention_workspace(const combo_cross_attention_t* d, int 
   if (!desc_ok(d)) return -1;
   const Plan p = plan_of(*d);
   const long long rows = (long long)d->B * d->Hq * d->Lq;
-  if (!backward_pass) return p.fwd.splits > 1 ? p.fwd.splits * rows * (d->D + 1) * 4 : 0;
-  const long long dq = p.dq.splits > 1 ? p.dq.splits * rows * d->D : 0;
+  if (!backward_pass) return p.splits > 1 ? p.splits * rows * (d->D + 1) * 4 : 0;
+  const long long dq = p.splits > 1 ? p.splits * rows * d->D : 0;
   const long long dkv = p.row_splits > 1 ? 2ll * p.row_splits * d->B * d->Lk * d->Hk * d->D : 0;
   return ((dq > dkv ? dq : dkv) + rows) * 4;
 }
@@ -1191,10 +1200,10 @@ long long combo_cross_attention_workspace(const combo_cross_attention_t* d, int 
 int combo_cross_attention_forward(const combo_cross_attention_t* d, void* out, float* lse, void* workspace, combo_stream_t stream) {
   if (!desc_ok(d) || !out || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 31)) return COMBO_EINVAL;
   const Plan p = plan_of(*d);
-  if (p.fwd.splits > 1 && !workspace) return COMBO_EINVAL;
+  if (p.splits > 1 && !workspace) return COMBO_EINVAL;
   Args A = args_of(*d);
   A.out = out, A.lse = lse, A.part = static_cast<float*>(workspace);
-  if (p.fwd.splits > 1) A.part_lse = A.part + (long long)p.fwd.splits * d->B * d->Hq * d->Lq * d->D;
+  if (p.splits > 1) A.part_lse = A.part + (long long)p.splits * d->B * d->Hq * d->Lq * d->D;
   return d->dtype == 1 ? by_dim<__bf16>(A, p, false, (hipStream_t)stream) : by_dim<_Float16>(A, p, false, (hipStream_t)stream);
 }
 
