@@ -1111,14 +1111,14 @@ Plan plan_of(const combo_cross_attention_t& d) {
 
 bool desc_ok(const combo_cross_attention_t* d) {
   if (!d || !d->q || !d->k || !d->v || d->B <= 0 || d->Lq <= 0 || d->Lk <= 0 || d->Hq <= 0 || d->Hk <= 0 || d->Hq % d->Hk || d->D <= 0 || d->D > 128 ||
-      d->D % 8 || (d->dtype != 1 && d->dtype != 2) || !(d->scale > 0.f) || !std::isfinite(d->scale))
+      d->D % 8 || (d->dtype != 1 && d->dtype != 2) || !(d->scale > 0.f) || !std::isfinite(d->scale * 1.4427f))
     return false;
   if (((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15) return false;
   for (int i = 0; i < 3; ++i)
     if ((d->q_stride[i] | d->k_stride[i] | d->v_stride[i]) & 7 || d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0) return false;
   if (d->k_stride[1] > (1 << 22) || d->v_stride[1] > (1 << 22)) return false;  // (32-bit byte offsets inside a tile of 128 keys)
   const long long G = d->Hq / d->Hk;
-  return (long long)d->Lq * G < (1ll << 30) && d->Lk < (1 << 30) && (long long)d->B * d->Hq * (((long long)d->Lq + 127) / 128 + ((long long)d->Lk + 127) / 128) < (1 << 24);
+  return (long long)d->Lq * G < (1ll << 30) && d->Lk < (1 << 30) && (long long)d->B * d->Hq * (((long long)d->Lq + 127) / 128 + ((long long)d->Lk + 127) / 128) < (1 << 30);
 }
 
 Args args_of(const combo_cross_attention_t& d) {

@@ -67,6 +67,8 @@ def _channels_last(x):
 
 def _act_workspace(x, places, groups, code, backward):
     n = _lib.lib().combo_groupnorm_act_workspace(x.shape[0], places, x.shape[1], groups, code, backward)
+    if n < 0:
+        raise ValueError(f"group_norm_act: sizes the kernels do not take: {tuple(x.shape)}")
     return torch.empty(n, device=x.device, dtype=torch.float32) if n else None
 
 
@@ -130,6 +132,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
         raise TypeError(f"group_norm_act: x is {x.dtype}, takes float32, bfloat16 or float16")
     if groups < 1 or C < 1 or C % groups or C > MAX_CHANNELS:
         raise ValueError(f"group_norm_act: {C} channels in {groups} groups (the groups divide the channels, at most {MAX_CHANNELS})")
+    if not 0 <= eps < float("inf"):
+        raise ValueError(f"group_norm_act: eps {eps}")
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None:
             if tuple(p.shape) != (C,):

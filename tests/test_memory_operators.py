@@ -26,7 +26,7 @@ def test_group_norm_act_refusals():
     x = torch.zeros(2, 8, 3, 3).contiguous(memory_format=torch.channels_last)
     for bad in (lambda: group_norm_act(x[0], 2), lambda: group_norm_act(x, 3), lambda: group_norm_act(x, 0), lambda: group_norm_act(x, 2, activation="tanh"),
                 lambda: group_norm_act(x, 2, torch.ones(7)), lambda: group_norm_act(x, 2, None, torch.ones(8, 1)), lambda: group_norm_act(x.contiguous(), 2),
-                lambda: group_norm_act(x[:, :4], 2), lambda: group_norm_act(torch.zeros(1, 4100, 1, 1), 2)):
+                lambda: group_norm_act(x[:, :4], 2), lambda: group_norm_act(x, 2, eps=-1e-5), lambda: group_norm_act(x, 2, eps=float("nan")), lambda: group_norm_act(torch.zeros(1, 4100, 1, 1), 2)):
         with pytest.raises(ValueError):
             bad()
     for bad in (lambda: group_norm_act(x.double(), 2), lambda: group_norm_act(x, 2, torch.ones(8).half()), lambda: group_norm_act(x.int(), 2)):
@@ -91,7 +91,7 @@ def test_cross_attention_entry_points_refuse_without_a_launch():
     assert lib.combo_cross_attention_workspace(desc(), 0) == 0 and lib.combo_cross_attention_workspace(desc(), 1) >= 16
     for bad in (desc(q=0), desc(q=one + 2), desc(qs=(64, 32, 12)), desc(qs=(64, -32, 16)), desc(B=0), desc(Lq=0), desc(Lk=0), desc(Hk=3), desc(D=12),
                 desc(D=136), desc(dtype=0), desc(dtype=3), desc(scale=0.0), desc(scale=float("inf")), desc(scale=float("nan")), desc(Lq=1 << 30),
-                desc(B=1 << 24)):
+                desc(B=1 << 30), desc(scale=3e38)):
         assert lib.combo_cross_attention_workspace(bad, 0) == -1
         assert lib.combo_cross_attention_forward(bad, one, 0, one, 0) == 1
         assert lib.combo_cross_attention_backward(bad, one, one, one, one, one, one, one, 0) == 1
