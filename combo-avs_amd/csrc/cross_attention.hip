@@ -1109,6 +1109,8 @@ Plan plan_of(const combo_cross_attention_t& d) {
   return p;
 }
 
+constexpr long long kMaxGrid = 1 << 24;  // workgroups of 256 threads
+
 bool desc_ok(const combo_cross_attention_t* d) {
   if (!d || !d->q || !d->k || !d->v || d->B <= 0 || d->Lq <= 0 || d->Lk <= 0 || d->Hq <= 0 || d->Hk <= 0 || d->Hq % d->Hk || d->D <= 0 || d->D > 128 ||
       d->D % 8 || (d->dtype != 1 && d->dtype != 2) || !(d->scale > 0.f) || !std::isfinite(d->scale * 1.4427f))
@@ -1117,8 +1119,9 @@ bool desc_ok(const combo_cross_attention_t* d) {
   for (int i = 0; i < 3; ++i)
     if ((d->q_stride[i] | d->k_stride[i] | d->v_stride[i]) & 7 || d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0) return false;
   if (d->k_stride[1] > (1 << 22) || d->v_stride[1] > (1 << 22)) return false;  // (32-bit byte offsets inside a tile of 128 keys)
-  const long long G = d->Hq / d->Hk;
-  return (long long)d->Lq * G < (1ll << 30) && d->Lk < (1 << 30) && (long long)d->B * d->Hq * (((long long)d->Lq + 127) / 128 + ((long long)d->Lk + 127) / 128) < (1 << 30);
+  if ((long long)d->Lq * (d->Hq / d->Hk) >= (1ll << 30) || d->Lk >= (1 << 30)) return false;
+  const Plan p = plan_of(*d);  // (workgroups of the largest launches: a grid holds less than 2^32 threads)
+  return (long long)d->B * d->Hk * p.tiles * p.splits < kMaxGrid && (long long)d->B * d->Hk * p.key_tiles * p.row_splits < kMaxGrid;
 }
 
 Args args_of(const combo_cross_attention_t& d) {
@@ -1136,7 +1139,7 @@ Args args_of(const combo_cross_attention_t& d) {
 
 template <void (*kernel)(const Args)>
 int launch(long long grid, size_t lds, const Args& A, hipStream_t st) {
-  if (grid <= 0 || grid > 0x7fffffffll) return COMBO_EINVAL;
+  if (grid <= 0 || grid >= kMaxGrid) return COMBO_EINVAL;
   if (lds > 65536) {
     static ComboDevFlag ready;  // (one per kernel: it is the template's argument)
     if (!ready.is_set()) {
@@ -1226,7 +1229,7 @@ int combo_cross_attention_pack(const unsigned char* blocked, long long stride_b,
   if (!blocked || !bits || B <= 0 || H <= 0 || N <= 0 || Lk <= 0 || stride_b < 0 || stride_h < 0 || stride_n < 0 || stride_k < 0) return COMBO_EINVAL;
   const int W = (Lk + 31) / 32;
   const long long total = (long long)B * H * N * W, grid = blocks_of(total);
-  if (grid > 0x7fffffffll) return COMBO_EINVAL;
+  if (grid >= kMaxGrid) return COMBO_EINVAL;
   hipLaunchKernelGGL(cross_pack_kernel, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, blocked, stride_b, stride_h, stride_n, stride_k, H, N,
                      Lk, W, total, bits);
   return (int)hipGetLastError();

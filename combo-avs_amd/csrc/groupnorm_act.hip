@@ -616,9 +616,11 @@ int run(NormArgs& A, int dtype, int act_, bool back, uintptr_t all, hipStream_t 
   return by_width<_Float16>(A, act_, back, all, st);
 }
 
+// (B * lines bounds every grid: a launch holds less than 2^32 threads)
 bool shape_ok(int B, int HW, int C, int G, int dtype, int act_) {
-  return B > 0 && HW > 0 && C > 0 && C <= kMaxC && G > 0 && C % G == 0 && dtype >= 0 && dtype <= 2 && act_ >= 0 && act_ <= 3 &&
-         (long long)B * C < 0x7fffffffll && B <= (1 << 22);
+  if (B <= 0 || HW <= 0 || C <= 0 || C > kMaxC || G <= 0 || C % G || dtype < 0 || dtype > 2 || act_ < 0 || act_ > 3) return false;
+  const int lines = (C * (dtype == 0 ? 4 : 2) + 127) / 128;
+  return (long long)B * C < 0x7fffffffll && B <= (1 << 22) && (long long)B * lines < (1 << 24);
 }
 
 }  // namespace

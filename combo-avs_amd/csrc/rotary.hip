@@ -131,7 +131,7 @@ int launch(RotaryArgs& A, hipStream_t st) {
   A.items_magic = magic(A.items);
   A.head_magic = magic(A.per_head);
   const long long grid = (A.tokens + A.T - 1) / A.T;
-  if (grid > 0x7fffffffll) return COMBO_EINVAL;
+  if (grid >= (1 << 24)) return COMBO_EINVAL;  // (a launch holds less than 2^32 threads)
   const size_t lds = (size_t)A.T * (A.D / 2) * sizeof(float2);
 #define COMBO_GO(V_) hipLaunchKernelGGL((rotary_kernel<T, V_>), dim3((unsigned)grid), dim3(256), lds, st, A)
   switch (V) {

@@ -48,6 +48,7 @@ def test_entry_points_refuse_bad_arguments_without_a_launch():
     assert all(rc == 1 for rc in (rotary(D=7), rotary(D=2), rotary(D=258), rotary(axes=0), rotary(axes=9), rotary(pos_type=4), rotary(dtype=3),
                                   rotary(B=0), rotary(x=0), rotary(x=4098), rotary(H=1 << 25)))
     assert lib.combo_groupnorm_act_workspace(1, 9, 8, 3, 0, 0) == -1 and lib.combo_groupnorm_act_workspace(1, 9, 4104, 2, 0, 0) == -1
+    assert lib.combo_groupnorm_act_workspace(1 << 18, 1, 4096, 2, 0, 0) == -1  # more workgroups than a launch holds
     assert lib.combo_groupnorm_act_workspace(2, 9, 8, 2, 0, 0) == 0 and lib.combo_groupnorm_act_workspace(2, 9, 8, 2, 0, 1) == 40
     assert lib.combo_groupnorm_act_workspace(2, 9000, 64, 2, 0, 0) > 0
     assert lib.combo_groupnorm_act_forward(one, 0, 0, 2, 9000, 64, 2, 1e-5, 0, 0, 0, one, one, one, 0) == 1  # two launches need their workspace
@@ -91,7 +92,7 @@ def test_cross_attention_entry_points_refuse_without_a_launch():
     assert lib.combo_cross_attention_workspace(desc(), 0) == 0 and lib.combo_cross_attention_workspace(desc(), 1) >= 16
     for bad in (desc(q=0), desc(q=one + 2), desc(qs=(64, 32, 12)), desc(qs=(64, -32, 16)), desc(B=0), desc(Lq=0), desc(Lk=0), desc(Hk=3), desc(D=12),
                 desc(D=136), desc(dtype=0), desc(dtype=3), desc(scale=0.0), desc(scale=float("inf")), desc(scale=float("nan")), desc(Lq=1 << 30),
-                desc(B=1 << 30), desc(scale=3e38)):
+                desc(B=1 << 24), desc(B=1 << 30), desc(scale=3e38)):
         assert lib.combo_cross_attention_workspace(bad, 0) == -1
         assert lib.combo_cross_attention_forward(bad, one, 0, one, 0) == 1
         assert lib.combo_cross_attention_backward(bad, one, one, one, one, one, one, one, 0) == 1
