@@ -541,33 +541,6 @@ __global__ void __launch_bounds__(256, 2) cross_wide_kernel(const Args A) {
   }
 }
 
-// joins the splits of a row: 8 values a thread
-template <typename T>
-__global__ void __launch_bounds__(256) cross_join_kernel(const Args A) {
-  const int per = A.D / 8;
-  const long long total = (long long)A.B * A.Hk * A.rows, i = blockIdx.x * 256ll + threadIdx.x;
-  const long long at = fast_div(i, per);
-  if (at >= total) return;
-  const int d = (int)(i - at * per) * 8;
-  float top = -kInf, sum = 0.f;
-  for (int s = 0; s < A.splits; ++s) top = fmaxf(top, A.part_lse[s * total + at]);
-  const float base = top == -kInf ? 0.f : top;
-  f32x8 x = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < A.splits; ++s) {
-    const float w = __builtin_amdgcn_exp2f(A.part_lse[s * total + at] - base);
-    sum += w;
-    const f32x8 y = *reinterpret_cast<const f32x8*>(A.part + (s * total + at) * A.D + d);
-    x += y * w;
-  }
-  const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-  const int r = (int)(at % A.rows);
-  const long long bh = at / A.rows;
-  const int hk = (int)(bh % A.Hk), b = (int)(bh / A.Hk);
-  const Row row(A, hk, r);
-  *reinterpret_cast<typename Type<T>::x8*>(static_cast<T*>(A.out) + row.packed(A, b) + d) = __builtin_convertvector(x * f, typename Type<T>::x8);
-  if (A.lse && d == 0) A.lse[at] = sum > 0.f ? base + log2f(sum) : (sum == 0.f ? kInf : sum);
-}
-
 // ---- backward -----------------------------------------------------------------------------------------------------------------
 
 // o . do of this lane's row as the diagonal of a product: the same order of summation as do . v, so a row that sees one key has ds = 0 exactly
@@ -782,23 +755,6 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
       for (int d = 0; d < DP / 32; ++d) put_row(o, acc[d], A.scale, 32 * d, A.D, half);
     }
   }
-}
-
-// sums the splits of dq
-template <typename T>
-__global__ void __launch_bounds__(256) cross_dq_sum_kernel(const Args A) {
-  const int per = A.D / 8;
-  const long long total = (long long)A.B * A.Hk * A.rows, i = blockIdx.x * 256ll + threadIdx.x;
-  const long long at = fast_div(i, per);
-  if (at >= total) return;
-  const int d = (int)(i - at * per) * 8;
-  f32x8 x = *reinterpret_cast<const f32x8*>(A.part + at * A.D + d);
-  for (int s = 1; s < A.splits; ++s) x += *reinterpret_cast<const f32x8*>(A.part + (s * total + at) * A.D + d);
-  const int r = (int)(at % A.rows);
-  const long long bh = at / A.rows;
-  const Row row(A, (int)(bh % A.Hk), r);
-  *reinterpret_cast<typename Type<T>::x8*>(static_cast<T*>(A.out) + row.packed(A, (int)(bh / A.Hk)) + d) =
-      __builtin_convertvector(x * A.scale, typename Type<T>::x8);
 }
 
 // dk, dv: a wave owns 32 keys, the workgroup walks the rows of all G heads.  Score tiles are rows x keys here (a lane owns a key), so they are
@@ -1043,13 +999,100 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
   }
 }
 
-// sums the splits of dk and dv: 8 values a thread
+// ---- the splits of a row joined, 8 values (a vector) at a time ------------------------------------------------------------------
+// A load's latency is ~0.65 us, and a thread that walks 64 splits one by one takes 42 us.  So P lanes share the splits of a vector, four loads
+// in flight each (the vectors of a wave stay side by side, the lanes of one lie 64 / P apart), and a tree over the lanes ends it: 4.1 us for 64
+// splits of 4 x 8 rows, 6.0 for 128, little more than a launch.
+
+__host__ __device__ inline int lanes_of(int splits) {
+  int P = 1;
+  while (P < 32 && 4 * P < splits) P *= 2;
+  return P;
+}
+
+struct Share {
+  int P, apart, first;  // lanes of a vector, their distance, this lane's first split
+  long long vector;
+  __device__ explicit Share(int splits) {
+    const int lane = threadIdx.x & 63;
+    P = lanes_of(splits), apart = 64 / P, first = lane / apart;
+    vector = (blockIdx.x * 256ll + threadIdx.x) / 64 * apart + lane % apart;
+  }
+  // sum of the vectors at from + s * step over the splits s, each times weight(s)
+  template <typename F>
+  __device__ f32x8 sum(const float* from, long long step, int splits, F weight) const {
+    f32x8 x = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s0 = first; s0 < splits; s0 += 4 * P) {
+      f32x8 y[4];
+      float w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int s = min(s0 + u * P, splits - 1);
+        y[u] = *reinterpret_cast<const f32x8*>(from + s * step);
+        w[u] = weight(s);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (s0 + u * P < splits) x += y[u] * w[u];
+    }
+    for (int o = apart; o < 64; o *= 2)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] += __shfl_xor(x[i], o);
+    return x;
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) cross_join_kernel(const Args A) {
+  const int per = A.D / 8;
+  const long long total = (long long)A.B * A.Hk * A.rows;
+  const Share mine(A.splits);
+  const bool on = mine.vector < total * per;
+  const long long i = on ? mine.vector : 0, at = fast_div(i, per);
+  const int d = (int)(i - at * per) * 8;
+  const float* lse = A.part_lse + at;
+  float top = -kInf, sum = 0.f;
+#pragma unroll 4
+  for (int s = mine.first; s < A.splits; s += mine.P) top = fmaxf(top, lse[s * total]);
+  for (int o = mine.apart; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+  const float base = top == -kInf ? 0.f : top;
+#pragma unroll 4
+  for (int s = mine.first; s < A.splits; s += mine.P) sum += __builtin_amdgcn_exp2f(lse[s * total] - base);
+  for (int o = mine.apart; o < 64; o *= 2) sum += __shfl_xor(sum, o);
+  const f32x8 x = mine.sum(A.part + at * A.D + d, total * A.D, A.splits, [&](int s) { return __builtin_amdgcn_exp2f(lse[s * total] - base); });
+  if (!on || mine.first) return;
+  const float f = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  const long long bh = at / A.rows;
+  const Row row(A, (int)(bh % A.Hk), (int)(at % A.rows));
+  *reinterpret_cast<typename Type<T>::x8*>(static_cast<T*>(A.out) + row.packed(A, (int)(bh / A.Hk)) + d) =
+      __builtin_convertvector(x * f, typename Type<T>::x8);
+  if (A.lse && d == 0) A.lse[at] = sum > 0.f ? base + log2f(sum) : (sum == 0.f ? kInf : sum);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) cross_dq_sum_kernel(const Args A) {
+  const int per = A.D / 8;
+  const long long total = (long long)A.B * A.Hk * A.rows;
+  const Share mine(A.splits);
+  const bool on = mine.vector < total * per;
+  const long long i = on ? mine.vector : 0, at = fast_div(i, per);
+  const int d = (int)(i - at * per) * 8;
+  const f32x8 x = mine.sum(A.part + at * A.D + d, total * A.D, A.splits, [](int) { return 1.f; });
+  if (!on || mine.first) return;
+  const long long bh = at / A.rows;
+  const Row row(A, (int)(bh % A.Hk), (int)(at % A.rows));
+  *reinterpret_cast<typename Type<T>::x8*>(static_cast<T*>(A.out) + row.packed(A, (int)(bh / A.Hk)) + d) =
+      __builtin_convertvector(x * A.scale, typename Type<T>::x8);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) cross_dkv_sum_kernel(const Args A) {
-  const long long all = (long long)A.B * A.Lk * A.Hk * A.D, i = (blockIdx.x * 256ll + threadIdx.x) * 8;
-  if (i >= 2 * all) return;
-  f32x8 x = *reinterpret_cast<const f32x8*>(A.part + i);
-  for (int s = 1; s < A.splits; ++s) x += *reinterpret_cast<const f32x8*>(A.part + 2 * s * all + i);
+  const long long all = (long long)A.B * A.Lk * A.Hk * A.D;
+  const Share mine(A.splits);
+  const bool on = mine.vector * 8 < 2 * all;
+  const long long i = on ? mine.vector * 8 : 0;
+  const f32x8 x = mine.sum(A.part + i, 2 * all, A.splits, [](int) { return 1.f; });
+  if (!on || mine.first) return;
   T* o = i < all ? static_cast<T*>(A.dk) + i : static_cast<T*>(A.dv) + (i - all);
   *reinterpret_cast<typename Type<T>::x8*>(o) = __builtin_convertvector(x, typename Type<T>::x8);
 }
@@ -1109,6 +1152,8 @@ Plan plan_of(const combo_cross_attention_t& d) {
   return p;
 }
 
+long long blocks_of(long long items) { return (items + 255) / 256; }
+
 constexpr long long kMaxGrid = 1 << 24;  // workgroups of 256 threads
 
 bool desc_ok(const combo_cross_attention_t* d) {
@@ -1152,14 +1197,12 @@ int launch(long long grid, size_t lds, const Args& A, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-long long blocks_of(long long items) { return (items + 255) / 256; }
-
 template <typename T, int DP>
 int forward(Args& A, const Plan& p, hipStream_t st) {
   A.tiles = p.tiles, A.splits = p.splits;
   const long long grid = (long long)A.B * A.Hk * A.splits * A.tiles;
   int rc = p.rows == 32 ? launch<cross_few_kernel<T, DP>>(grid, Few<DP>::LDS, A, st) : launch<cross_wide_kernel<T, DP>>(grid, Wide<DP>::LDS, A, st);
-  if (rc == 0 && A.splits > 1) rc = launch<cross_join_kernel<T>>(blocks_of((long long)A.B * A.Hk * A.rows * (A.D / 8)), 0, A, st);
+  if (rc == 0 && A.splits > 1) rc = launch<cross_join_kernel<T>>(blocks_of((long long)A.B * A.Hk * A.rows * (A.D / 8) * lanes_of(A.splits)), 0, A, st);
   return rc;
 }
 
@@ -1169,13 +1212,13 @@ int backward(Args& A, const Plan& p, hipStream_t st) {
   A.tiles = p.tiles, A.splits = p.splits;
   const long long grid = (long long)A.B * A.Hk * A.splits * A.tiles;
   int rc = p.rows == 32 ? launch<cross_dq_kernel<T, DP, 1>>(grid, Dq<DP, 1>::LDS, A, st) : launch<cross_dq_kernel<T, DP, 4>>(grid, Dq<DP, 4>::LDS, A, st);
-  if (rc == 0 && A.splits > 1) rc = launch<cross_dq_sum_kernel<T>>(blocks_of((long long)A.B * A.Hk * A.rows * (A.D / 8)), 0, A, st);
+  if (rc == 0 && A.splits > 1) rc = launch<cross_dq_sum_kernel<T>>(blocks_of((long long)A.B * A.Hk * A.rows * (A.D / 8) * lanes_of(A.splits)), 0, A, st);
   if (rc) return rc;
   if (!A.dk) return 0;
   A.part = part;
   A.tiles = p.key_tiles, A.splits = p.row_splits;
   rc = launch<cross_dkv_kernel<T, DP>>((long long)A.B * A.Hk * A.splits * A.tiles, Bwd<T, DP>::LDS, A, st);
-  if (rc == 0 && A.splits > 1) rc = launch<cross_dkv_sum_kernel<T>>(blocks_of((long long)A.B * A.Lk * A.Hk * (A.D / 8) * 2), 0, A, st);
+  if (rc == 0 && A.splits > 1) rc = launch<cross_dkv_sum_kernel<T>>(blocks_of((long long)A.B * A.Lk * A.Hk * (A.D / 8) * 2 * lanes_of(A.splits)), 0, A, st);
   return rc;
 }
 
