@@ -1130,13 +1130,17 @@ struct Plan {
   int key_tiles, row_splits;  // dk, dv
 };
 
-// Workgroups over the other axis when there are few: two for each of the 256 CUs, at least one tile each.  From one workgroup a CU on, a short axis
-// is left whole: 320 workgroups of 13 tiles take 26.8 us, and in two halves 22.7 us and a join of 4.2 us and one more launch.
-int pick_splits(long long groups, int tiles) {
-  long long s = groups >= 256 && tiles < 32 ? 1 : (512 + groups - 1) / groups;
+// Workgroups over the other axis when there are few: two for each of the 256 CUs, at least one tile each.  Left whole are a walk of a few tiles,
+// which costs no more than the join and saves a launch (8 x 100 rows over 256 keys of 64: 7.5 against 9.7 us replayed, 13.8 against 17.3 called;
+// one row of 4 x 8 over 784 keys of 32: 8.6 against 9.6, 14.2 against 18.2; replayed, 8 tiles of 64: 10.8 against 10.3, 8 of 128: 16.6 against
+// 11.3), and from one workgroup a CU on a short axis: 320 workgroups of 13 tiles take 26.8 us, and in two halves 22.7 us and a join of 4.2 us and
+// one more launch.
+int pick_splits(long long groups, int tiles, int D) {
+  if (tiles <= (D > 64 ? 4 : 7) || (groups >= 256 && tiles < 32)) return 1;
+  long long s = (512 + groups - 1) / groups;
   if (s > tiles) s = tiles;
   if (s > 128) s = 128;
-  return s < 1 ? 1 : (int)s;
+  return (int)s;
 }
 
 Plan plan_of(const combo_cross_attention_t& d) {
@@ -1146,9 +1150,14 @@ Plan plan_of(const combo_cross_attention_t& d) {
   p.rows = rows <= 32 ? 32 : 128;
   p.tiles = (int)((rows + p.rows - 1) / p.rows);
   const int kt = p.rows == 32 ? 128 : 64;
-  p.splits = pick_splits(bh * p.tiles, (d.Lk + kt - 1) / kt);
+  const int key_tiles = (d.Lk + kt - 1) / kt;
+  p.splits = pick_splits(bh * p.tiles, key_tiles, d.D);
+  // few rows, which cost what it takes to read the keys: shares of 32 tiles and more are halved, so that the workgroups of the longer samples do
+  // not finish alone (16 x 8 x 16384 keys of 128: all as long 208 -> 198 us, 5.4 TB/s; 25 to 100 % as long 165 -> 153; shares of 8 tiles, 8 x 8
+  // x 4096 keys: 26.6 against 27.5)
+  if (p.rows == 32 && key_tiles >= 32 * p.splits) p.splits *= 2;
   p.key_tiles = (d.Lk + 127) / 128;
-  p.row_splits = pick_splits(bh * p.key_tiles, (int)((rows + 31) / 32));
+  p.row_splits = pick_splits(bh * p.key_tiles, (int)((rows + 31) / 32), d.D);
   return p;
 }
 

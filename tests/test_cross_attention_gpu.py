@@ -248,3 +248,12 @@ def test_runs_repeat_bit_for_bit_on_streams_and_in_graphs():
             twin.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(step(), held2))
+
+
+@pytest.mark.parametrize("B,Lk,Hq,Hk,D", [(1, 9000, 2, 1, 128), (1, 17000, 3, 3, 64), (2, 1030, 4, 2, 16), (64, 4100, 8, 8, 8)])
+def test_single_tokens_over_long_states(B, Lk, Hq, Hk, D):
+    """shares of a row by the dozen, shares that a short sample leaves empty, and halved shares"""
+    q, k, v = made(B, 1, Lk, Hq, Hk, D, torch.bfloat16)
+    check(q, k, v)
+    lengths = torch.randint(0, Lk + 1, (B,), generator=torch.Generator().manual_seed(B), dtype=torch.int32)
+    check(q, k, v, lengths=lengths.cuda(), blocked=(torch.rand(B, 1, 1, Lk, generator=torch.Generator().manual_seed(Lk)) < 0.3).cuda())
