@@ -222,7 +222,7 @@ __device__ __forceinline__ Range split_range(int len, int splits, int s, int til
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------
 
-// few rows (at most 32): the four waves hold the same rows and share the keys of a tile, 32 each
+// few rows, in blocks of 32: the four waves hold the same rows and share the keys of a tile, 32 each
 template <int DP>
 struct Few {
   static constexpr int KW = 4, KT = 32 * KW, TILE = KT * Tile<DP>::PITCH;
@@ -250,8 +250,10 @@ __global__ void __launch_bounds__(256, 2) cross_few_kernel(const Args A) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   T* Kt = reinterpret_cast<T*>(lds);
   T* Vt = Kt + F::TILE;
-  const int lane = threadIdx.x & 63, kw = threadIdx.x >> 6, half = lane >> 5, r = lane & 31;
+  const int lane = threadIdx.x & 63, kw = threadIdx.x >> 6, half = lane >> 5, c = lane & 31;
   int id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int r = id % A.tiles * 32 + c;
+  id /= A.tiles;
   const int split = id % A.splits;
   id /= A.splits;
   const int hk = id % A.Hk, b = id / A.Hk, len = length_of(A, b);
@@ -334,15 +336,15 @@ __global__ void __launch_bounds__(256, 2) cross_few_kernel(const Args A) {
   __syncthreads();
   float top = -kInf, sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < F::KW; ++w) top = fmaxf(top, ml[w * 32 + r]);
+  for (int w = 0; w < F::KW; ++w) top = fmaxf(top, ml[w * 32 + c]);
   const float base = top == -kInf ? 0.f : top * A.c;
 #pragma unroll
-  for (int w = 0; w < F::KW; ++w) sum += ml[(F::KW + w) * 32 + r] * __builtin_amdgcn_exp2f(ml[w * 32 + r] * A.c - base);
+  for (int w = 0; w < F::KW; ++w) sum += ml[(F::KW + w) * 32 + c] * __builtin_amdgcn_exp2f(ml[w * 32 + c] * A.c - base);
   const float f = sum > 0.f ? __builtin_amdgcn_exp2f(m * A.c - base) / sum : (sum == 0.f ? 0.f : sum);
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) part[(kw * DP + 32 * d + reg_row(i, half)) * 32 + r] = acc[d][i] * f;
+    for (int i = 0; i < 16; ++i) part[(kw * DP + 32 * d + reg_row(i, half)) * 32 + c] = acc[d][i] * f;
   __syncthreads();
   if (r >= A.rows) return;
   const long long at = ((long long)b * A.Hk + hk) * A.rows + r, total = (long long)A.B * A.Hk * A.rows;
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(256, 2) cross_few_kernel(const Args A) {
     for (int j = 0; j < 4; ++j) {
       x[j] = 0.f;
 #pragma unroll
-      for (int w = 0; w < F::KW; ++w) x[j] += part[(w * DP + d + j) * 32 + r];
+      for (int w = 0; w < F::KW; ++w) x[j] += part[(w * DP + d + j) * 32 + c];
     }
     if (A.splits > 1) {
       *reinterpret_cast<float4*>(A.part + (split * total + at) * A.D + d) = make_float4(x[0], x[1], x[2], x[3]);
@@ -560,7 +562,7 @@ __device__ __forceinline__ float row_dot(const typename Type<T>::x8 (&o)[DP / 16
 
 // dq: the walk over the keys again, p from the saved lse; per tile two score-sized products and the one with K.  The scores of tile t + 1 are
 // formed in the same basic block in which the vector unit turns those of tile t into ds, so there are three buffers (t, t + 1, and t + 2 filling).
-// RW = 4: a wave owns 32 rows; RW = 1 (at most 32 rows): the waves share the keys of a tile.
+// RW = 4: a wave owns 32 rows; RW = 1 (blocks of 32 rows): the waves share the keys of a tile.
 template <int DP, int RW>
 struct Dq {
   static constexpr int KW = 4 / RW, KB = RW == 4 && DP < 128 ? 2 : 1, KT = 32 * KB * KW, RT = 32 * RW, TILE = KT * Tile<DP>::PITCH;
@@ -1143,14 +1145,19 @@ int pick_splits(long long groups, int tiles, int D) {
   return (int)s;
 }
 
-Plan plan_of(const combo_cross_attention_t& d) {
+// Blocks of 128 rows read a key once for all of them; blocks of 32 are four times as many.  So these are taken for 32 rows, and where 128 would
+// leave CUs idle or need a join and 32 need none (forward, dq, each with its join, 128 against 32 rows a block): 8 x 8 x 100 rows over 784 keys of 32
+// 14.4, 14.9 against 10.1, 10.5 us; 16 x 8 x 100 over 784 of 64 19.9, 22.7 against 15.6, 18.2; 2 x 8 x 512 over 1024 of 128 26.8, 30.3 against
+// 18.5, 22.9.  Not for dq of more than 64 dimensions, with one workgroup a CU, beyond one round of them: 16 x 8 x 100 over 784 of 128 32.0 against
+// 40.4.  Longer walks stay with 128: 1 x 8 x 1024 over 8192 of 128 62.4, 72.2 against 93.5, 158.
+Plan plan_of(const combo_cross_attention_t& d, bool back) {
   Plan p;
   const int G = d.Hq / d.Hk;
-  const long long rows = (long long)d.Lq * G, bh = (long long)d.B * d.Hk;
-  p.rows = rows <= 32 ? 32 : 128;
+  const long long rows = (long long)d.Lq * G, bh = (long long)d.B * d.Hk, small = bh * ((rows + 31) / 32);
+  const bool whole = bh * ((rows + 127) / 128) < 256 && pick_splits(small, (d.Lk + 127) / 128, d.D) == 1 && !(back && d.D > 64 && small > 256);
+  p.rows = rows <= 32 || whole ? 32 : 128;
   p.tiles = (int)((rows + p.rows - 1) / p.rows);
-  const int kt = p.rows == 32 ? 128 : 64;
-  const int key_tiles = (d.Lk + kt - 1) / kt;
+  const int kt = p.rows == 32 ? 128 : 64, key_tiles = (d.Lk + kt - 1) / kt;
   p.splits = pick_splits(bh * p.tiles, key_tiles, d.D);
   // few rows, which cost what it takes to read the keys: shares of 32 tiles and more are halved, so that the workgroups of the longer samples do
   // not finish alone (16 x 8 x 16384 keys of 128: all as long 208 -> 198 us, 5.4 TB/s; 25 to 100 % as long 165 -> 153; shares of 8 tiles, 8 x 8
@@ -1174,8 +1181,11 @@ bool desc_ok(const combo_cross_attention_t* d) {
     if ((d->q_stride[i] | d->k_stride[i] | d->v_stride[i]) & 7 || d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0) return false;
   if (d->k_stride[1] > (1 << 22) || d->v_stride[1] > (1 << 22)) return false;  // (32-bit byte offsets inside a tile of 128 keys)
   if ((long long)d->Lq * (d->Hq / d->Hk) >= (1ll << 30) || d->Lk >= (1 << 30)) return false;
-  const Plan p = plan_of(*d);  // (workgroups of the largest launches: a grid holds less than 2^32 threads)
-  return (long long)d->B * d->Hk * p.tiles * p.splits < kMaxGrid && (long long)d->B * d->Hk * p.key_tiles * p.row_splits < kMaxGrid;
+  for (const bool back : {false, true}) {  // (workgroups of the largest launches: a grid holds less than 2^32 threads)
+    const Plan p = plan_of(*d, back);
+    if ((long long)d->B * d->Hk * p.tiles * p.splits >= kMaxGrid || (long long)d->B * d->Hk * p.key_tiles * p.row_splits >= kMaxGrid) return false;
+  }
+  return true;
 }
 
 Args args_of(const combo_cross_attention_t& d) {
@@ -1244,7 +1254,7 @@ extern "C" {
 
 long long combo_cross_attention_workspace(const combo_cross_attention_t* d, int backward_pass) {
   if (!desc_ok(d)) return -1;
-  const Plan p = plan_of(*d);
+  const Plan p = plan_of(*d, backward_pass);
   const long long rows = (long long)d->B * d->Hq * d->Lq;
   if (!backward_pass) return p.splits > 1 ? p.splits * rows * (d->D + 1) * 4 : 0;
   const long long dq = p.splits > 1 ? p.splits * rows * d->D : 0;
@@ -1254,7 +1264,7 @@ long long combo_cross_attention_workspace(const combo_cross_attention_t* d, int 
 
 int combo_cross_attention_forward(const combo_cross_attention_t* d, void* out, float* lse, void* workspace, combo_stream_t stream) {
   if (!desc_ok(d) || !out || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 31)) return COMBO_EINVAL;
-  const Plan p = plan_of(*d);
+  const Plan p = plan_of(*d, false);
   if (p.splits > 1 && !workspace) return COMBO_EINVAL;
   Args A = args_of(*d);
   A.out = out, A.lse = lse, A.part = static_cast<float*>(workspace);
@@ -1267,7 +1277,7 @@ int combo_cross_attention_backward(const combo_cross_attention_t* d, const void*
   if (!desc_ok(d) || !out || !lse || !dout || !workspace || !dq || (!dk) != (!dv) ||
       (((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) || ((uintptr_t)workspace & 31))
     return COMBO_EINVAL;
-  const Plan p = plan_of(*d);
+  const Plan p = plan_of(*d, true);
   Args A = args_of(*d);
   A.o = out, A.lse = const_cast<float*>(lse), A.dout = dout, A.out = dq, A.dk = dk, A.dv = dv;
   const long long bytes = combo_cross_attention_workspace(d, 1);

@@ -257,3 +257,16 @@ def test_single_tokens_over_long_states(B, Lk, Hq, Hk, D):
     check(q, k, v)
     lengths = torch.randint(0, Lk + 1, (B,), generator=torch.Generator().manual_seed(B), dtype=torch.int32)
     check(q, k, v, lengths=lengths.cuda(), blocked=(torch.rand(B, 1, 1, Lk, generator=torch.Generator().manual_seed(Lk)) < 0.3).cuda())
+
+
+@pytest.mark.parametrize("B,Lq,Lk,Hq,Hk,D,dtype", [(16, 129, 300, 8, 8, 32, torch.bfloat16), (16, 130, 161, 8, 8, 64, torch.float16), (16, 150, 100, 8, 8, 80, torch.bfloat16),
+                                                   (32, 70, 77, 8, 4, 40, torch.float16), (16, 129, 130, 8, 8, 128, torch.bfloat16), (9, 1000, 31, 4, 4, 24, torch.bfloat16)])
+def test_blocks_that_fill_the_chip(B, Lq, Lk, Hq, Hk, D, dtype):
+    """at least 256 blocks of 128 rows, whose keys are not split"""
+    q, k, v = made(B, Lq, Lk, Hq, Hk, D, dtype)
+    gen = torch.Generator().manual_seed(D)
+    lengths = torch.randint(0, Lk + 1, (B,), generator=gen, dtype=torch.int32)
+    lengths[:3] = torch.tensor([Lk, 0, 1])
+    check(q, k, v)
+    check(q, k, v, lengths=lengths.cuda(), blocked=(torch.rand(B, 1, Lq, Lk, generator=gen) < 0.6).cuda())
+    check(q, k, v, lengths=lengths.cuda(), blocked=(torch.rand(B, 1, 1, Lk, generator=gen) < 0.5).cuda())
