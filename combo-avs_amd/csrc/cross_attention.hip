@@ -1132,39 +1132,41 @@ struct Plan {
   int key_tiles, row_splits;  // dk, dv
 };
 
-// Workgroups over the other axis when there are few: two for each of the 256 CUs, at least one tile each.  Left whole are a walk of a few tiles,
-// which costs no more than the join and saves a launch (8 x 100 rows over 256 keys of 64: 7.5 against 9.7 us replayed, 13.8 against 17.3 called;
-// one row of 4 x 8 over 784 keys of 32: 8.6 against 9.6, 14.2 against 18.2; replayed, 8 tiles of 64: 10.8 against 10.3, 8 of 128: 16.6 against
-// 11.3), and from one workgroup a CU on a short axis: 320 workgroups of 13 tiles take 26.8 us, and in two halves 22.7 us and a join of 4.2 us and
-// one more launch.
-int pick_splits(long long groups, int tiles, int D) {
+// Splits of the other axis when there are few workgroups: as many as `slots`, one round of what the chip holds, allow (4 x 10 x 4096 rows against 77
+// keys: dk, dv in 13 shares are 520 workgroups and take 26.2 us, in 12 21.8; 3 x 8 x 300 rows over 5000 keys of 128: 24 shares 49.0, 21 38.9).
+// Left whole are a walk of a few tiles, which costs no more than the join and saves a launch (8 x 100 rows over 256 keys of 64: 7.5 against 9.7 us
+// replayed, 13.8 against 17.3 called; one row of 4 x 8 over 784 keys of 32: 8.6 against 9.6, 14.2 against 18.2; replayed, 8 tiles of 64: 10.8
+// against 10.3, 8 of 128: 16.6 against 11.3), and from one workgroup a CU on a short axis: 320 workgroups of 13 tiles take 26.8 us, and in two
+// halves 22.7 us and a join of 4.2 us and one more launch.
+int pick_splits(long long groups, int tiles, int D, int slots) {
   if (tiles <= (D > 64 ? 4 : 7) || (groups >= 256 && tiles < 32)) return 1;
-  long long s = (512 + groups - 1) / groups;
+  long long s = slots / groups;
   if (s > tiles) s = tiles;
   if (s > 128) s = 128;
-  return (int)s;
+  return s < 1 ? 1 : (int)s;
 }
 
 // Blocks of 128 rows read a key once for all of them; blocks of 32 are four times as many.  So these are taken for 32 rows, and where 128 would
 // leave CUs idle or need a join and 32 need none (forward, dq, each with its join, 128 against 32 rows a block): 8 x 8 x 100 rows over 784 keys of 32
 // 14.4, 14.9 against 10.1, 10.5 us; 16 x 8 x 100 over 784 of 64 19.9, 22.7 against 15.6, 18.2; 2 x 8 x 512 over 1024 of 128 26.8, 30.3 against
-// 18.5, 22.9.  Not for dq of more than 64 dimensions, with one workgroup a CU, beyond one round of them: 16 x 8 x 100 over 784 of 128 32.0 against
+// 18.5, 22.9; 1 x 8 x 1024 over 2048 of 128 32.8, 36.3 against 30.9, 35.9.  Not for dq of more than 64 dimensions, with one workgroup a CU, beyond one round of them: 16 x 8 x 100 over 784 of 128 32.0 against
 // 40.4.  Longer walks stay with 128: 1 x 8 x 1024 over 8192 of 128 62.4, 72.2 against 93.5, 158.
 Plan plan_of(const combo_cross_attention_t& d, bool back) {
   Plan p;
   const int G = d.Hq / d.Hk;
   const long long rows = (long long)d.Lq * G, bh = (long long)d.B * d.Hk, small = bh * ((rows + 31) / 32);
-  const bool whole = bh * ((rows + 127) / 128) < 256 && pick_splits(small, (d.Lk + 127) / 128, d.D) == 1 && !(back && d.D > 64 && small > 256);
+  const bool whole = bh * ((rows + 127) / 128) < 256 && d.Lk <= 2048 && pick_splits(small, (d.Lk + 127) / 128, d.D, 512) == 1 &&
+                     !(back && d.D > 64 && small > 256);
   p.rows = rows <= 32 || whole ? 32 : 128;
   p.tiles = (int)((rows + p.rows - 1) / p.rows);
   const int kt = p.rows == 32 ? 128 : 64, key_tiles = (d.Lk + kt - 1) / kt;
-  p.splits = pick_splits(bh * p.tiles, key_tiles, d.D);
+  p.splits = pick_splits(bh * p.tiles, key_tiles, d.D, 512);  // (two workgroups a CU)
   // few rows, which cost what it takes to read the keys: shares of 32 tiles and more are halved, so that the workgroups of the longer samples do
   // not finish alone (16 x 8 x 16384 keys of 128: all as long 208 -> 198 us, 5.4 TB/s; 25 to 100 % as long 165 -> 153; shares of 8 tiles, 8 x 8
   // x 4096 keys: 26.6 against 27.5)
   if (p.rows == 32 && key_tiles >= 32 * p.splits) p.splits *= 2;
   p.key_tiles = (d.Lk + 127) / 128;
-  p.row_splits = pick_splits(bh * p.key_tiles, (int)((rows + 31) / 32), d.D);
+  p.row_splits = pick_splits(bh * p.key_tiles, (int)((rows + 31) / 32), d.D, d.D > 64 ? 256 : 512);  // (one, two: 31.4 us in 512, 24.6 in 256)
   return p;
 }
 
