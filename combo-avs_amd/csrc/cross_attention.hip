@@ -63,9 +63,10 @@ __device__ __forceinline__ int length_of(const Args& A, int b) {
 }
 
 // row-major LDS tile of 16-bit values.  The pitch is an odd number p of 16-byte chunks with p = 3, 7 or 9 (mod 16): 16 rows at the same chunk (a
-// b128 operand read) start in 16 different chunks of the 64 banks, and 4 rows x 2 neighbouring chunks (16 lanes of a transposed read) in 8, so
-// neither conflicts (SQ_LDS_BANK_CONFLICT: 0), and every address is one lane register plus an immediate; a swizzle by exclusive-or costs a
-// register or an instruction per operand, and the kernels are short of both.
+// b128 operand read) start in 16 different chunks of the 64 banks, and 4 rows x 2 neighbouring chunks (16 lanes of a transposed read) in 8, and
+// every address is one lane register plus an immediate.  Conflicts are left in a quarter of the LDS cycles (SQ_LDS_BANK_CONFLICT); a swizzle by
+// exclusive-or has none, but costs a register or an instruction per operand, of which the kernels are short: forward at 64 x 4096 x 4096 x 128
+// 1272 us with the swizzle, 997 with the pitch.
 template <int DP>
 struct Tile {
   static constexpr int PITCH = DP == 32 ? 56 : (DP == 64 ? 72 : 152);
@@ -222,7 +223,8 @@ __device__ __forceinline__ Range split_range(int len, int splits, int s, int til
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------
 
-// few rows, in blocks of 32: the four waves hold the same rows and share the keys of a tile, 32 each
+// few rows, in blocks of 32: the four waves hold the same rows and share the keys of a tile, 32 each.  Bound by the read of K and V: 16 x 8 x 16384
+// keys of 128 (1.07 GB) 198 us = 5.4 TB/s, ragged lengths 153; a single round of workgroups (4 x 8 x 784 of 32) 8 us, which are latency.
 template <int DP>
 struct Few {
   static constexpr int KW = 4, KT = 32 * KW, TILE = KT * Tile<DP>::PITCH;
@@ -378,8 +380,13 @@ __global__ void __launch_bounds__(256, 2) cross_few_kernel(const Args A) {
 
 // many rows: a wave owns 32, the workgroup 128.  A wave's matrix instructions and its softmax would take turns (a score costs ~5 vector
 // instructions of 4 cycles for D / 8 cycles of the matrix pipe), so three tiles are in work at once: while the vector unit turns the scores of
-// tile t into probabilities, the matrix pipe forms the scores of tile t + 1 and adds the product of tile t - 1 - in one basic block, interleaved
-// by hand.  K and V have two LDS buffers each and one barrier a tile: K runs one tile ahead, V one behind.
+// tile t into probabilities, the matrix pipe forms the scores of tile t + 1 and adds the product of tile t - 1, all in one basic block, where the
+// compiler mixes them.  K and V have two LDS buffers each and one barrier a tile: K runs one tile ahead, V one behind.  The loads stand at the head
+// of a step (at its end: 720 us instead of 600).
+// Bound by the matrix and vector instructions together and, with both at work, by the power that lowers the clock to ~1.9 GHz: 64 x 4096 x 4096 x
+// 128 592 us = 930 TFLOP/s (one tile at a time: 997), 32 x 4099 x 15680 x 64 760 to 860 us (at 64 dimensions a score's exponential weighs twice as
+// much; without it 6 % less, without operand reads from LDS 18 %).  Tried without gain: 64 rows a wave (spills), more waves of smaller tiles, loads
+// two tiles ahead, no running maximum, chains of maxima and sums.
 template <int DP>
 struct Wide {
   static constexpr int KB = DP == 128 ? 1 : 2, KT = 32 * KB, RT = 128, TILE = KT * Tile<DP>::PITCH;
@@ -465,8 +472,8 @@ __global__ void __launch_bounds__(256, 2) cross_wide_kernel(const Args A) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
     top = other_max(top);
-    // the reference point only moves once a score passes it by 2^8 in the result: p then stays under 2^8, exact in every type, and the
-    // accumulators are rescaled a few times in all instead of once a tile
+    // the reference point only moves once a score passes it by 2^8 in the result: p then stays under 2^8, in the range of every type, and
+    // the accumulators are rescaled a few times in all instead of once a tile
     if (__any((top - run.m) * A.c > 8.f)) {  // (-inf against -inf: NaN, no)
       add_values(vbuf + other);
 #pragma unroll
@@ -562,6 +569,8 @@ __device__ __forceinline__ float row_dot(const typename Type<T>::x8 (&o)[DP / 16
 
 // dq: the walk over the keys again, p from the saved lse; per tile two score-sized products and the one with K.  The scores of tile t + 1 are
 // formed in the same basic block in which the vector unit turns those of tile t into ds, so there are three buffers (t, t + 1, and t + 2 filling).
+// 64 x 4096 x 4096 x 128: 750 to 800 us = 1.05 PFLOP/s (6 S D), like the forward pass at its power limit (tiles one at a time: 1395; loads at the
+// step's end: 815).
 // RW = 4: a wave owns 32 rows; RW = 1 (blocks of 32 rows): the waves share the keys of a tile.
 template <int DP, int RW>
 struct Dq {
@@ -760,10 +769,11 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
 }
 
 // dk, dv: a wave owns 32 keys, the workgroup walks the rows of all G heads.  Score tiles are rows x keys here (a lane owns a key), so they are
-// the B operands of dV^T = dO^T P and dK^T = Q^T dS; lse and delta of a tile's rows lie in LDS.
+// the B operands of dV^T = dO^T P and dK^T = Q^T dS; lse and delta of a tile's rows lie in LDS.  Tiles of 32 rows: of 64, at 32 dimensions, they took
+// all 256 registers and 40 x 8 x 100 rows and 784 keys 35.6 us instead of 30.7 (4 x 8 x 2000 and 2000 keys, enough work a wave: 60.8 and 65.0).
 template <typename T, int DP>
 struct Bwd {
-  static constexpr int KT = 128, RT = DP == 32 ? 64 : 32;
+  static constexpr int KT = 128, RT = 32;
   static constexpr int TILE = 2 * RT * Tile<DP>::PITCH * 2, SIDE = 2 * RT * 4 + 4 * RT * 4;  // Q and dO; lse, delta and the four waves' mask words
   static constexpr int BUF = TILE + SIDE, LDS = 3 * BUF;
 };
@@ -795,38 +805,36 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
   const T* q = reinterpret_cast<const T*>(A.q) + b * A.qb;
   const T* g = static_cast<const T*>(A.dout);
   const long long side = ((long long)b * A.Hk + hk) * A.rows;
-  constexpr int N = F::RT * (DP / 8) / 256, STEP = 256 / (DP / 8);
-  // a thread's vectors of a tile; where G divides a tile's rows they move on by the same distance from tile to tile
+  // a thread's vectors of a tile, of Q and of dO by turns (one vector: half of the threads each); where G divides a tile's rows they move on by the
+  // same distance from tile to tile
+  constexpr int N = 2 * F::RT * (DP / 8) / 256, STEP = 256 / (DP / 8);
   const bool even = F::RT % A.G == 0 && A.D == DP;
   const int c = threadIdx.x % (DP / 8), x0 = threadIdx.x / (DP / 8);
   const int to = Tile<DP>::at(x0, c);
-  long long qat[N], gat[N];
+  const long long qstep = F::RT / A.G * A.qn, gstep = (long long)(F::RT / A.G) * A.Hq * A.D;
+  auto of_q = [&](int i) { return N == 1 ? x0 < F::RT : i % 2 == 0; };
+  auto row_of = [&](int i) { return N == 1 ? x0 % F::RT : x0 + STEP * (i / 2); };
+  long long at[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const Row row(A, hk, x0 + STEP * i);
-    qat[i] = row.n * A.qn + row.h * A.qh + c * 8;
-    gat[i] = row.packed(A, b) + c * 8;
+    const Row row(A, hk, row_of(i));
+    at[i] = (of_q(i) ? row.n * A.qn + row.h * A.qh : row.packed(A, b)) + c * 8;
   }
-  const long long qstep = F::RT / A.G * A.qn, gstep = (long long)(F::RT / A.G) * A.Hq * A.D;
-  u32x4 rq[N], rg[N];
+  u32x4 held[N];
   float rl = 0.f;
   unsigned rm = 0u;
   auto fetch = [&](int rt) {
     if (even && (rt + 1) * F::RT <= A.rows) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        rq[i] = *reinterpret_cast<const u32x4*>(q + rt * qstep + qat[i]);
-        rg[i] = *reinterpret_cast<const u32x4*>(g + rt * gstep + gat[i]);
-      }
+      for (int i = 0; i < N; ++i) held[i] = *reinterpret_cast<const u32x4*>((of_q(i) ? q + rt * qstep : g + rt * gstep) + at[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int r = rt * F::RT + x0 + STEP * i;
-        rq[i] = rg[i] = u32x4{0u, 0u, 0u, 0u};
+        const int r = rt * F::RT + row_of(i);
+        held[i] = u32x4{0u, 0u, 0u, 0u};
         if (r < A.rows && c * 8 < A.D) {
           const Row row(A, hk, r);
-          rq[i] = *reinterpret_cast<const u32x4*>(q + row.n * A.qn + row.h * A.qh + c * 8);
-          rg[i] = *reinterpret_cast<const u32x4*>(g + row.packed(A, b) + c * 8);
+          held[i] = *reinterpret_cast<const u32x4*>(of_q(i) ? q + row.n * A.qn + row.h * A.qh + c * 8 : g + row.packed(A, b) + c * 8);
         }
       }
     }
@@ -847,10 +855,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
   auto park = [&](char* buf) {
     T* Qt = reinterpret_cast<T*>(buf);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      *reinterpret_cast<u32x4*>(Qt + to + i * STEP * Tile<DP>::PITCH) = rq[i];
-      *reinterpret_cast<u32x4*>(Qt + (F::RT + i * STEP) * Tile<DP>::PITCH + to) = rg[i];
-    }
+    for (int i = 0; i < N; ++i) *reinterpret_cast<u32x4*>(Qt + to + (i / 2 * STEP + i % 2 * F::RT) * Tile<DP>::PITCH) = held[i];
     if (threadIdx.x < 2 * F::RT) reinterpret_cast<float*>(buf + F::TILE)[threadIdx.x] = rl;
     if (A.bits && threadIdx.x < 4 * F::RT) reinterpret_cast<unsigned*>(buf + F::TILE + 2 * F::RT * 4)[threadIdx.x] = rm;
   };
@@ -871,7 +876,8 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
   };
   // The compiler places an LDS read right before the instruction that needs it, and with one or two waves on a SIMD its latency then shows at every
   // product.  So a tile is worked in four stages that nothing is moved across; a stage's products take operands that the stage before has read,
-  // and its vector instructions do not wait for its own products:
+  // and its vector instructions do not wait for its own products (64 x 4096 x 4096 x 128: 1750 us as one block, now 1270 to 1380 = 830 TFLOP/s of
+  // 8 S D, one wave a SIMD):
   //     dP of tile t               | p = exp2(S)               | reads Q of tile t + 1
   //     S of tile t + 1            | ds = p (dP - delta)       | reads dO^T of tile t
   //     dV += dO^T p               |                           | reads Q^T of tile t
@@ -980,9 +986,9 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) ak[d] = av[d] = zero16();
   }
-  const long long at = (((long long)b * A.Lk + key) * A.Hk + hk) * A.D, all = (long long)A.B * A.Lk * A.Hk * A.D;
+  const long long here = (((long long)b * A.Lk + key) * A.Hk + hk) * A.D, all = (long long)A.B * A.Lk * A.Hk * A.D;
   if (A.splits > 1) {
-    float* o = A.part + 2 * split * all + at;
+    float* o = A.part + 2 * split * all + here;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -995,8 +1001,8 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
   } else {
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) {
-      put_row(static_cast<T*>(A.dk) + at, ak[d], A.scale, 32 * d, A.D, half);
-      put_row(static_cast<T*>(A.dv) + at, av[d], 1.f, 32 * d, A.D, half);
+      put_row(static_cast<T*>(A.dk) + here, ak[d], A.scale, 32 * d, A.D, half);
+      put_row(static_cast<T*>(A.dv) + here, av[d], 1.f, 32 * d, A.D, half);
     }
   }
 }
@@ -1099,7 +1105,7 @@ __global__ void __launch_bounds__(256) cross_dkv_sum_kernel(const Args A) {
   *reinterpret_cast<typename Type<T>::x8*>(o) = __builtin_convertvector(x, typename Type<T>::x8);
 }
 
-// ---- the mask as bits: one word per 32 keys, so the kernels read 1/8 of a byte mask's traffic, and that by whole words ----------
+// ---- the mask as bits: one word per 32 keys, so the kernels read 1/8 of a byte mask's traffic, and that by whole words (40 x 100 x 784: 5.9 us) -----
 __global__ void __launch_bounds__(256) cross_pack_kernel(const unsigned char* blocked, long long sb, long long sh, long long sn, long long sk,
                                                          int H, int N, int Lk, int W, long long total, unsigned* bits) {
   const long long i = blockIdx.x * 256ll + threadIdx.x;
@@ -1166,7 +1172,8 @@ Plan plan_of(const combo_cross_attention_t& d, bool back) {
   // x 4096 keys: 26.6 against 27.5)
   if (p.rows == 32 && key_tiles >= 32 * p.splits) p.splits *= 2;
   p.key_tiles = (d.Lk + 127) / 128;
-  p.row_splits = pick_splits(bh * p.key_tiles, (int)((rows + 31) / 32), d.D, d.D > 64 ? 256 : 512);  // (one, two: 31.4 us in 512, 24.6 in 256)
+  const int slots = d.D > 64 ? 256 : (d.D > 32 ? 512 : 768);  // (one, two, three a CU; 2 x 8 x 512 rows and 1024 keys of 128 in 512 shares: 31.4 us, in 256: 24.6)
+  p.row_splits = pick_splits(bh * p.key_tiles, (int)((rows + 31) / 32), d.D, slots);
   return p;
 }
 
