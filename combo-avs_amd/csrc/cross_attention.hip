@@ -859,20 +859,17 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
     if (threadIdx.x < 2 * F::RT) reinterpret_cast<float*>(buf + F::TILE)[threadIdx.x] = rl;
     if (A.bits && threadIdx.x < 4 * F::RT) reinterpret_cast<unsigned*>(buf + F::TILE + 2 * F::RT * 4)[threadIdx.x] = rm;
   };
-  constexpr int RB = F::RT / 32;
-  auto mask = [&](const char* buf, f32x16 (&s)[RB]) {
+  auto mask = [&](const char* buf, f32x16& s) {
     if (!A.bits) return;
     const unsigned* Mt = reinterpret_cast<const unsigned*>(buf + F::TILE + 2 * F::RT * 4) + wave * F::RT;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+    for (int i = 0; i < 16; i += 4) {
+      const uint4 w = *reinterpret_cast<const uint4*>(Mt + reg_row(i, half));
+      const unsigned w4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const uint4 w = *reinterpret_cast<const uint4*>(Mt + 32 * rb + reg_row(i, half));
-        const unsigned w4[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if ((w4[j] >> (lane & 31)) & 1) s[rb][i + j] = -kInf;
-      }
+      for (int j = 0; j < 4; ++j)
+        if ((w4[j] >> (lane & 31)) & 1) s[i + j] = -kInf;
+    }
   };
   // The compiler places an LDS read right before the instruction that needs it, and with one or two waves on a SIMD its latency then shows at every
   // product.  So a tile is worked in four stages that nothing is moved across; a stage's products take operands that the stage before has read,
@@ -883,47 +880,37 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
   //     dV += dO^T p               |                           | reads Q^T of tile t
   //     dK += Q^T ds               |                           | reads dO and lse of tile t + 1
   constexpr int ND = DP / 16, NT = DP / 32;
-  typedef x8 Rows[RB][ND];      // operands of a product over the head dimension
-  typedef x8 Cols[RB][2][NT];   // operands of a product over the tile's rows
+  typedef x8 Rows[ND];     // operands of a product over the head dimension
+  typedef x8 Cols[2][NT];  // operands of a product over the tile's rows
   auto read_rows = [&](const T* Xt, Rows& x) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) x[rb][d] = operand<T, DP>(Xt, 32 * rb, d);
+    for (int d = 0; d < ND; ++d) x[d] = operand<T, DP>(Xt, 0, d);
   };
   auto read_cols = [&](const T* Xt, Cols& x) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+    for (int st = 0; st < 2; ++st)
 #pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int d = 0; d < NT; ++d) x[rb][st][d] = operand_t<T, DP>(Xt, 32 * rb + 16 * st, 32 * d);
+      for (int d = 0; d < NT; ++d) x[st][d] = operand_t<T, DP>(Xt, 16 * st, 32 * d);
   };
   auto q_tile = [&](int buf) { return reinterpret_cast<const T*>(lds + buf); };
   auto g_tile = [&](int buf) { return reinterpret_cast<const T*>(lds + buf) + F::RT * Tile<DP>::PITCH; };
-  auto over_rows = [&](const Rows& x, const x8 (&y)[ND], f32x16 (&o)[RB]) {
+  auto over_rows = [&](const Rows& x, const x8 (&y)[ND], f32x16& o) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[rb] = Type<T>::mfma(x[rb][d], y[d], d ? o[rb] : zero16());
+    for (int d = 0; d < ND; ++d) o = Type<T>::mfma(x[d], y[d], d ? o : zero16());
   };
-  auto over_cols = [&](const Cols& x, const x8 (&y)[RB][2], f32x16 (&o)[NT]) {
+  auto over_cols = [&](const Cols& x, const x8 (&y)[2], f32x16 (&o)[NT]) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+    for (int st = 0; st < 2; ++st)
 #pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int d = 0; d < NT; ++d) o[d] = Type<T>::mfma(x[rb][st][d], y[rb][st], o[d]);
+      for (int d = 0; d < NT; ++d) o[d] = Type<T>::mfma(x[st][d], y[st], o[d]);
   };
-  // a value per row (lse or delta) for this lane's 16 rows of each block
-  auto read_side = [&](const float* side_, f32x16 (&x)[RB]) {
+  // a value per row (lse or delta) for this lane's 16 rows
+  auto read_side = [&](const float* side_, f32x16& x) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const float4 y = *reinterpret_cast<const float4*>(side_ + 32 * rb + reg_row(i, half));
-        x[rb][i] = y.x, x[rb][i + 1] = y.y, x[rb][i + 2] = y.z, x[rb][i + 3] = y.w;
-      }
+    for (int i = 0; i < 16; i += 4) {
+      const float4 y = *reinterpret_cast<const float4*>(side_ + reg_row(i, half));
+      x[i] = y.x, x[i + 1] = y.y, x[i + 2] = y.z, x[i + 3] = y.w;
+    }
   };
   auto lse_of = [&](int buf) { return reinterpret_cast<const float*>(lds + buf + F::TILE); };
   if (lo < hi) {
@@ -934,7 +921,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
       park(lds + F::BUF);
     }
     __syncthreads();
-    f32x16 s[RB], dp[RB], x[RB], L[RB];
+    f32x16 s, dp, x, L;
     Rows rows;
     Cols cols, cols2;
     read_rows(q_tile(0), rows);
@@ -949,26 +936,20 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
       over_rows(rows, v, dp);
       Rows next;
       read_rows(q_tile(bn), next);  // (behind the last tile: what lies in the buffer, not used)
-      x8 p[RB][2], ds[RB][2];
+      x8 p[2], ds[2];
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[rb][i] = __builtin_amdgcn_exp2f(fmaf(s[rb][i], A.c, -L[rb][i]));
-        // p, and ds below, are rounded to the tensor's type for the products (half a step relative to each)
-        p[rb][0] = pack<T>(x[rb], 0);
-        p[rb][1] = pack<T>(x[rb], 1);
-      }
+      for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(s[i], A.c, -L[i]));
+      // p, and ds below, are rounded to the tensor's type for the products (half a step relative to each)
+      p[0] = pack<T>(x, 0);
+      p[1] = pack<T>(x, 1);
       read_side(lse_of(bt) + F::RT, L);  // delta
       __builtin_amdgcn_sched_barrier(0);
       over_rows(next, k, s);
       read_cols(g_tile(bt), cols);
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[rb][i] *= dp[rb][i] - L[rb][i];
-        ds[rb][0] = pack<T>(x[rb], 0);
-        ds[rb][1] = pack<T>(x[rb], 1);
-      }
+      for (int i = 0; i < 16; ++i) x[i] *= dp[i] - L[i];
+      ds[0] = pack<T>(x, 0);
+      ds[1] = pack<T>(x, 1);
       __builtin_amdgcn_sched_barrier(0);
       over_cols(cols, p, av);
       read_cols(q_tile(bt), cols2);
@@ -1155,8 +1136,9 @@ int pick_splits(long long groups, int tiles, int D, int slots) {
 // Blocks of 128 rows read a key once for all of them; blocks of 32 are four times as many.  So these are taken for 32 rows, and where 128 would
 // leave CUs idle or need a join and 32 need none (forward, dq, each with its join, 128 against 32 rows a block): 8 x 8 x 100 rows over 784 keys of 32
 // 14.4, 14.9 against 10.1, 10.5 us; 16 x 8 x 100 over 784 of 64 19.9, 22.7 against 15.6, 18.2; 2 x 8 x 512 over 1024 of 128 26.8, 30.3 against
-// 18.5, 22.9; 1 x 8 x 1024 over 2048 of 128 32.8, 36.3 against 30.9, 35.9.  Not for dq of more than 64 dimensions, with one workgroup a CU, beyond one round of them: 16 x 8 x 100 over 784 of 128 32.0 against
-// 40.4.  Longer walks stay with 128: 1 x 8 x 1024 over 8192 of 128 62.4, 72.2 against 93.5, 158.
+// 18.5, 22.9; 1 x 8 x 1024 over 2048 of 128 32.8, 36.3 against 30.9, 35.9.  Not for dq of more than 64 dimensions, with one workgroup a CU, beyond
+// one round of them: 16 x 8 x 100 over 784 of 128 32.0 against 40.4.  Longer walks stay with 128: 1 x 8 x 1024 over 8192 of 128 62.4, 72.2
+// against 93.5, 158.
 Plan plan_of(const combo_cross_attention_t& d, bool back) {
   Plan p;
   const int G = d.Hq / d.Hk;
@@ -1172,7 +1154,7 @@ Plan plan_of(const combo_cross_attention_t& d, bool back) {
   // x 4096 keys: 26.6 against 27.5)
   if (p.rows == 32 && key_tiles >= 32 * p.splits) p.splits *= 2;
   p.key_tiles = (d.Lk + 127) / 128;
-  const int slots = d.D > 64 ? 256 : (d.D > 32 ? 512 : 768);  // (one, two, three a CU; 2 x 8 x 512 rows and 1024 keys of 128 in 512 shares: 31.4 us, in 256: 24.6)
+  const int slots = d.D > 64 ? 256 : (d.D > 32 ? 512 : 768);  // (one, two, three a CU; 2 x 8 x 512 rows, 1024 keys of 128: 31.4 us in 512, 24.6 in 256)
   p.row_splits = pick_splits(bh * p.key_tiles, (int)((rows + 31) / 32), d.D, slots);
   return p;
 }
@@ -1239,14 +1221,17 @@ int backward(Args& A, const Plan& p, hipStream_t st) {
   float* part = A.part;
   A.tiles = p.tiles, A.splits = p.splits;
   const long long grid = (long long)A.B * A.Hk * A.splits * A.tiles;
-  int rc = p.rows == 32 ? launch<cross_dq_kernel<T, DP, 1>>(grid, Dq<DP, 1>::LDS, A, st) : launch<cross_dq_kernel<T, DP, 4>>(grid, Dq<DP, 4>::LDS, A, st);
-  if (rc == 0 && A.splits > 1) rc = launch<cross_dq_sum_kernel<T>>(blocks_of((long long)A.B * A.Hk * A.rows * (A.D / 8) * lanes_of(A.splits)), 0, A, st);
+  int rc = p.rows == 32 ? launch<cross_dq_kernel<T, DP, 1>>(grid, Dq<DP, 1>::LDS, A, st)
+                        : launch<cross_dq_kernel<T, DP, 4>>(grid, Dq<DP, 4>::LDS, A, st);
+  if (rc == 0 && A.splits > 1)
+    rc = launch<cross_dq_sum_kernel<T>>(blocks_of((long long)A.B * A.Hk * A.rows * (A.D / 8) * lanes_of(A.splits)), 0, A, st);
   if (rc) return rc;
   if (!A.dk) return 0;
   A.part = part;
   A.tiles = p.key_tiles, A.splits = p.row_splits;
   rc = launch<cross_dkv_kernel<T, DP>>((long long)A.B * A.Hk * A.splits * A.tiles, Bwd<T, DP>::LDS, A, st);
-  if (rc == 0 && A.splits > 1) rc = launch<cross_dkv_sum_kernel<T>>(blocks_of((long long)A.B * A.Lk * A.Hk * (A.D / 8) * 2 * lanes_of(A.splits)), 0, A, st);
+  if (rc == 0 && A.splits > 1)
+    rc = launch<cross_dkv_sum_kernel<T>>(blocks_of((long long)A.B * A.Lk * A.Hk * (A.D / 8) * 2 * lanes_of(A.splits)), 0, A, st);
   return rc;
 }
 

@@ -9,6 +9,8 @@
 //                result.  For maps whose slice per workgroup is small (the launch then costs more than the traffic).
 //   two launches partial statistics per (image, slice of tokens), then every workgroup of the second launch joins the partials of its own
 //                image - a few KB out of L2 - and writes its tokens.
+// 40 x 256 x 56 x 56 bf16 with SiLU (64 MB): forward 14 us for the statistics (4.6 TB/s) and 30 for the result (4.3), backward 32 for the sums (4.0)
+// and 38 for dx (5.0), where a copy reaches 5.15; 3 x 60 x 117 x 93 fp16 with GELU (3.9 MB): 7, 9, 9 and 9 us; one 256 x 7 x 7 frame: 6.5 us.
 // Statistics: a thread sums x - K and (x - K)^2 with K its own first value of the channel, in fp32, and hands on (mean, M2); these are
 // joined as M2 = sum M2_i + sum n_i (mean_i - mean)^2.  K is one of the values, so the shift's cancellation is at most n_thread * 2^-24 of M2
 // whatever the offset of the map (a plain sum of squares loses everything once mean^2 > 2^24 var).  All sums have a fixed order.

@@ -9,6 +9,7 @@
 // longer than the memory traffic.  Angles in 64 bits: position * frequency is formed in TURNS and reduced to [-1/2, 1/2] in double
 // (a position of 1e6 has 3 decimal digits of angle left in fp32); the reduced turn is rounded to fp32 (2^-25 of a turn, 2e-7 rad)
 // and goes through sincospi.  The products are fp32, rounded once to the tensor's type.
+// 8 x 15680 tokens of 8 x 32 bf16 (64 MB read, 64 written): 28 us = 4.6 TB/s; one token of 8 sequences, or 2 x 713: 4 us, a launch and the angles.
 #include "combo_common.h"
 
 namespace {
