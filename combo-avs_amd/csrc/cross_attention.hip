@@ -101,6 +101,15 @@ __device__ __forceinline__ typename Type<T>::x8 pack(const f32x16& p, int s) {
   return __builtin_convertvector(x, typename Type<T>::x8);
 }
 
+// what pack left off, itself rounded
+template <typename T>
+__device__ __forceinline__ typename Type<T>::x8 left_off(const f32x16& p, int s, const typename Type<T>::x8& packed) {
+  f32x8 x;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = p[8 * s + i] - (float)packed[i];
+  return __builtin_convertvector(x, typename Type<T>::x8);
+}
+
 __device__ __forceinline__ float other_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -321,9 +330,15 @@ __global__ void __launch_bounds__(256, 2) cross_few_kernel(const Args A) {
     }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
-      const x8 p = pack<T>(s, st);
+      // p in two pieces, a product each, and o is as exact as its own rounding (1.0 of that error, 1.2 to 1.4 in one piece): where the keys' read
+      // is what takes the time it costs nothing (16 x 8 x 4 rows over 16384 keys of 128: 195 and 196 us), else up to a tenth (15.8 and 17.4)
+      const x8 p = pack<T>(s, st), rest = left_off<T>(s, st, p);
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mfma(operand_t<T, DP>(Vt, 32 * kw + 16 * st, 32 * d), p, acc[d]);
+      for (int d = 0; d < DP / 32; ++d) {
+        const x8 values_t = operand_t<T, DP>(Vt, 32 * kw + 16 * st, 32 * d);
+        acc[d] = Type<T>::mfma(values_t, p, acc[d]);
+        acc[d] = Type<T>::mfma(values_t, rest, acc[d]);
+      }
     }
   }
   // the waves hold the same rows: join their maxima, sums and results
@@ -575,7 +590,7 @@ __device__ __forceinline__ float row_dot(const typename Type<T>::x8 (&o)[DP / 16
 template <int DP, int RW>
 struct Dq {
   static constexpr int KW = 4 / RW, KB = RW == 4 && DP < 128 ? 2 : 1, KT = 32 * KB * KW, RT = 32 * RW, TILE = KT * Tile<DP>::PITCH;
-  static constexpr int BUFS = RW == 4 ? 3 : 1, LDS = 2 * BUFS * TILE * 2;
+  static constexpr int BUFS = RW == 4 ? 3 : 1, TILES = 2 * BUFS * TILE * 2, LDS = TILES + (KW > 1 ? KW * 32 * 4 : 0);
   static_assert(KW == 1 || KW * 32 * DP * 4 <= 2 * TILE * 2, "the join of the waves fits the tiles");
 };
 
@@ -630,7 +645,6 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
     delta = row_dot<T, DP>(o, g);
   }
   const float lse = on ? A.lse[at] : kInf;
-  if (on && half == 0 && kw == 0 && split == 0) A.delta[at] = delta;
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) acc[d] = zero16();
@@ -649,8 +663,12 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
     }
   };
   // ds, rounded to the tensor's type for the product (half a step relative to each).  States that no query sees were staged as zeros, so dp is
-  // finite where p is zero by a length or a shared mask.
-  auto gradient = [&](const T* Vt, const f32x16 (&s)[KB], x8 (&ds)[KB][2]) {
+  // finite where p is zero by a length or a shared mask.  In blocks of 32 rows and up to 32 dimensions, where a product costs little, what the
+  // rounding left off follows in a product of its own: dq came out 1.45 to 1.55 times the error of its own rounding, most of it at 16 dimensions,
+  // and is now at 1.05 (40 x 8 x 100 rows over 784 keys of 32: 28 -> 33 us, 16 x 8 x 4 rows over 16384 of 128: 188 -> 196).
+  constexpr int PIECES = DP == 32 || RW == 1 ? 2 : 1;
+  typedef x8 Grad[KB][2][PIECES];
+  auto gradient = [&](const T* Vt, const f32x16 (&s)[KB], Grad& ds) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       f32x16 dp;
@@ -661,18 +679,44 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
       for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], A.c, -lse));
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] *= dp[i] - delta;
-      ds[kb][0] = pack<T>(x, 0);
-      ds[kb][1] = pack<T>(x, 1);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        ds[kb][st][0] = pack<T>(x, st);
+        if constexpr (PIECES == 2) ds[kb][st][1] = left_off<T>(x, st, ds[kb][st][0]);
+      }
     }
   };
-  auto add_keys = [&](const T* Kt, const x8 (&ds)[KB][2]) {
+  // Delta = o . do carries the rounding of o and of the probabilities that made it, and over few keys that is as large as the rounding of ds.
+  // Where this workgroup has the whole row in LDS, delta + sum_j p_j (dp_j - delta) takes its place: the same number without the roundings
+  // (16 keys: dq and dk 1.56 -> 1.44 times the error of one rounding; 77 keys: 1.46, 2048: 1.43).
+  const bool at_hand = keys.lo == 0 && keys.hi == len && steps <= (RW == 4 ? 2 : 1);
+  auto missing = [&](const T* Kt, const T* Vt, int k0) {
+    f32x16 s[KB];
+    scores(Kt, s);
+    mask(k0, s);
+    float sum = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      f32x16 dp;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) dp = Type<T>::mfma(operand<T, DP>(Vt, (kw * KB + kb) * 32, d), g[d], d ? dp : zero16());
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(s[kb][i], A.c, -lse)) * (dp[i] - delta);
+    }
+    bits.load(words, keys.lo + kw * KB * 32, len);
+    return both_sum(sum);
+  };
+  auto add_keys = [&](const T* Kt, const Grad& ds) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-          acc[d] = Type<T>::mfma(operand_t<T, DP>(Kt, (kw * KB + kb) * 32 + 16 * st, 32 * d), ds[kb][st], acc[d]);
+        for (int d = 0; d < DP / 32; ++d) {
+          const x8 keys_t = operand_t<T, DP>(Kt, (kw * KB + kb) * 32 + 16 * st, 32 * d);
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) acc[d] = Type<T>::mfma(keys_t, ds[kb][st][i], acc[d]);
+        }
   };
   bits.load(words, keys.lo + kw * KB * 32, len);
   if (RW == 1) {
@@ -683,8 +727,16 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
       sv.store(vbuf);
       if (t + 1 < steps) fetch(sk, sv, k0 + F::KT);
       __syncthreads();
+      if (at_hand) {
+        float* sums = reinterpret_cast<float*>(lds + F::TILES);
+        const float sum = missing(kbuf, vbuf, k0);
+        if (half == 0) sums[wave * 32 + lane] = sum;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < F::KW; ++w) delta += sums[w * 32 + (lane & 31)];
+      }
       f32x16 s[KB];
-      x8 ds[KB][2];
+      Grad ds;
       scores(kbuf, s);
       mask(k0, s);
       gradient(vbuf, s, ds);
@@ -698,6 +750,14 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
       v1.store(vbuf + F::TILE);
     }
     __syncthreads();
+    if (at_hand) {
+      float sum = missing(kbuf, vbuf, keys.lo);
+      if (steps > 1) {
+        bits.load(words, keys.lo + F::KT, len);
+        sum += missing(kbuf + F::TILE, vbuf + F::TILE, keys.lo + F::KT);
+      }
+      delta += sum;
+    }
     f32x16 s[KB];
     scores(kbuf, s);
     int kt = 0, kn = F::TILE, kf = 2 * F::TILE;  // K (and V) of tile t, t + 1, t + 2
@@ -706,7 +766,7 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
       if (t + 2 < steps) fetch(sk, sv, k0 + 2 * F::KT);
       __syncthreads();
       mask(k0, s);
-      x8 ds[KB][2];
+      Grad ds;
       gradient(vbuf + kt, s, ds);
       scores(kbuf + kn, s);  // (behind the last tile: what lies in the buffer, not used)
       add_keys(kbuf + kt, ds);
@@ -716,6 +776,7 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
       kt = kn, kn = kf, kf = x;
     }
   }
+  if (on && half == 0 && kw == 0 && split == 0) A.delta[at] = delta;
   auto store = [&](int d, const float (&x)[4]) {
     if (d >= A.D) return;
     if (A.splits > 1) {
@@ -842,6 +903,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
       const int r = rt * F::RT + threadIdx.x % F::RT;
       const float* from = threadIdx.x < F::RT ? A.lse : A.delta;
       rl = r < A.rows ? from[side + r] : (threadIdx.x < F::RT ? kInf : 0.f);
+      if (std::is_same_v<T, _Float16> && threadIdx.x < F::RT) rl -= 12.f;  // (below)
     }
     if (A.bits) {
       const int x = threadIdx.x, r = rt * F::RT + x % F::RT, w = tile * 4 + x / F::RT;
@@ -904,6 +966,10 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
 #pragma unroll
       for (int d = 0; d < NT; ++d) o[d] = Type<T>::mfma(x[st][d], y[st], o[d]);
   };
+  // fp16 holds p as 2^12 p: over thousands of keys most of p is under 2^-14, where the type runs out of digits (16384 keys: dv 1.55 -> 1.41 times
+  // the error of one rounding); p <= 1 stays in range.  lse is read 12 less, dv ends with the reverse.
+  constexpr bool half_type = std::is_same_v<T, _Float16>;
+  constexpr float kUp = half_type ? 4096.f : 1.f, kDown = 1.f / kUp;
   // a value per row (lse or delta) for this lane's 16 rows
   auto read_side = [&](const float* side_, f32x16& x) {
 #pragma unroll
@@ -947,7 +1013,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
       over_rows(next, k, s);
       read_cols(g_tile(bt), cols);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= dp[i] - L[i];
+      for (int i = 0; i < 16; ++i) x[i] *= half_type ? (dp[i] - L[i]) * kDown : dp[i] - L[i];
       ds[0] = pack<T>(x, 0);
       ds[1] = pack<T>(x, 1);
       __builtin_amdgcn_sched_barrier(0);
@@ -977,13 +1043,13 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
         const int dd = 32 * d + reg_row(i, half);
         if (dd >= A.D) continue;
         *reinterpret_cast<float4*>(o + dd) = make_float4(ak[d][i] * A.scale, ak[d][i + 1] * A.scale, ak[d][i + 2] * A.scale, ak[d][i + 3] * A.scale);
-        *reinterpret_cast<float4*>(o + all + dd) = make_float4(av[d][i], av[d][i + 1], av[d][i + 2], av[d][i + 3]);
+        *reinterpret_cast<float4*>(o + all + dd) = make_float4(av[d][i] * kDown, av[d][i + 1] * kDown, av[d][i + 2] * kDown, av[d][i + 3] * kDown);
       }
   } else {
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) {
       put_row(static_cast<T*>(A.dk) + here, ak[d], A.scale, 32 * d, A.D, half);
-      put_row(static_cast<T*>(A.dv) + here, av[d], 1.f, 32 * d, A.D, half);
+      put_row(static_cast<T*>(A.dv) + here, av[d], kDown, 32 * d, A.D, half);
     }
   }
 }

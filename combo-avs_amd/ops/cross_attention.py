@@ -104,9 +104,10 @@ def cross_attention(q, k, v, kv_lengths=None, blocked=None, scale=None):
     kv_lengths [B] (int32 / int64, on the GPU): sample b has its first kv_lengths[b] states, clamped to 0 .. Lk.  blocked: bool,
     broadcastable to [B, Hq, Lq, Lk], True = this query does not see this key.  A query that sees no key gets zeros and passes no
     gradient.  States behind a sample's length, and states that a mask shared by all queries and heads blocks, may hold anything; a state
-    that only some queries are kept from has to be finite.  scale: positive, D ** -0.5 by default.  Probabilities are rounded to the
-    tensors' type before the second product, as are the score gradients in the backward pass; sums, statistics and gradients
-    accumulate in fp32 in a fixed order (runs repeat bit for bit); in fp16 a score gradient beyond 65504 becomes infinite."""
+    that only some queries are kept from has to be finite.  scale: positive, D ** -0.5 by default.  Probabilities enter the
+    second product in the tensors' type (in two pieces where few rows make the matrix work cheap), as do the score gradients in the
+    backward pass; sums, statistics and gradients accumulate in fp32 in a fixed order (runs repeat bit for bit); in fp16 a score
+    gradient beyond 65504 overflows."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"cross_attention: q [B, Lq, Hq, D], k and v [B, Lk, Hk, D]: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     B, Lq, Hq, D = q.shape

@@ -270,3 +270,20 @@ def test_blocks_that_fill_the_chip(B, Lq, Lk, Hq, Hk, D, dtype):
     check(q, k, v)
     check(q, k, v, lengths=lengths.cuda(), blocked=(torch.rand(B, 1, Lq, Lk, generator=gen) < 0.6).cuda())
     check(q, k, v, lengths=lengths.cuda(), blocked=(torch.rand(B, 1, 1, Lk, generator=gen) < 0.5).cuda())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,Lq,Lk,D", [(8, 4, 512, 4, 64), (8, 4, 512, 16, 16), (2, 4, 512, 40, 128), (2, 4, 512, 300, 16), (8, 4, 8, 2000, 64), (1, 1, 300, 16384, 64)])
+def test_errors_are_those_of_two_roundings(B, H, Lq, Lk, D, dtype):
+    """Root mean squares: a result carries its own rounding and that of one operand (p or ds), independent and as large where mantissas are spread
+    alike: sqrt(2) times the error of rounding the exact result, and an eighth more for mantissas that are not."""
+    from combo_avs_amd.ops.cross_attention import cross_attention
+    gen = torch.Generator().manual_seed(Lk + D)
+    q, k, v, dout = (torch.randn(B, L, H, D, generator=gen).to(dtype) for L in (Lq, Lk, Lk, Lq))
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    out = cross_attention(*leaves)
+    got = [out.detach()] + list(torch.autograd.grad(out, leaves, dout.cuda()))
+    want, _ = defined(q, k, v, None, None, D ** -0.5, dout)
+    for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
+        off, own = (a.double().cpu() - b).norm(), (b.to(dtype).double() - b).norm()
+        assert off <= 1.125 * 2 ** 0.5 * own, (name, float(off / own))
