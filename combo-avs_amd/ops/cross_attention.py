@@ -119,8 +119,8 @@ def cross_attention(q, k, v, kv_lengths=None, blocked=None, scale=None):
     if Hk < 1 or Hq % Hk:
         raise ValueError(f"cross_attention: {Hq} query heads on {Hk} key heads")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < float("inf"):
-        raise ValueError(f"cross_attention: scale {scale}: positive and finite")
+    if not 1e-37 < scale < 2e38:
+        raise ValueError(f"cross_attention: scale {scale}: positive and finite in fp32")
     if kv_lengths is not None:
         if kv_lengths.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"cross_attention: kv_lengths are {kv_lengths.dtype}, takes int32 or int64")

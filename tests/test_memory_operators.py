@@ -66,7 +66,8 @@ def test_cross_attention_refusals():
     for bad in (lambda: cross_attention(q[0], k, k), lambda: cross_attention(q, k, k[:, :4]), lambda: cross_attention(q[:1], k, k),
                 lambda: cross_attention(q, k[..., :8], k[..., :8]), lambda: cross_attention(q[..., :12], k[..., :12], k[..., :12]),
                 lambda: cross_attention(q[:, :, :3], k, k), lambda: cross_attention(q, k[:, :, :0], k[:, :, :0]), lambda: cross_attention(q, k, k, scale=0.0),
-                lambda: cross_attention(q, k, k, scale=-1.0), lambda: cross_attention(q, k, k, scale=float("nan")), lambda: cross_attention(q, k, k, n[:1]),
+                lambda: cross_attention(q, k, k, scale=-1.0), lambda: cross_attention(q, k, k, scale=float("nan")),
+                lambda: cross_attention(q, k, k, scale=1e39), lambda: cross_attention(q, k, k, scale=1e-60), lambda: cross_attention(q, k, k, n[:1]),
                 lambda: cross_attention(q, k, k, blocked=torch.zeros(2, 1, 3, 4, dtype=torch.bool)),
                 lambda: cross_attention(q, k, k, blocked=torch.zeros(3, 5, dtype=torch.bool)),
                 lambda: cross_attention(q, k, k, blocked=torch.zeros(2, 2, 3, 5, dtype=torch.bool)),
