@@ -73,7 +73,7 @@ def _act_workspace(x, places, groups, code, backward):
 
 
 def _act_forward(x, weight, bias, groups, eps, act, keep=False):
-    """-> (y, mean and rstd [2, B, groups] for the backward pass or None)"""
+    """weight, bias: contiguous fp32 or None -> (y, mean and rstd [2, B, groups] for the backward pass or None)"""
     B, C, places = x.shape[0], x.shape[1], x.shape[2:].numel()
     y = torch.empty_like(x)  # (preserves channels_last)
     stats = torch.empty(2, B, groups, device=x.device, dtype=torch.float32) if keep else None
@@ -88,12 +88,21 @@ def _act_forward(x, weight, bias, groups, eps, act, keep=False):
     return y, stats
 
 
+def _param(p):
+    return None if p is None else p.float().contiguous()
+
+
+def _as_given(dw, db, types):
+    return [g if g is None or g.dtype == t else g.to(t) for g, t in zip((dw, db), types)]
+
+
 class _GroupNormAct(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
+        ctx.groups, ctx.act, ctx.types = groups, act, [None if p is None else p.dtype for p in (weight, bias)]
+        weight, bias = _param(weight), _param(bias)
         y, stats = _act_forward(x, weight, bias, groups, eps, act, True)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.groups, ctx.act = groups, act
         return y
 
     @staticmethod
@@ -106,7 +115,7 @@ class _GroupNormAct(Function):
         dw = new(C, device=x.device, dtype=torch.float32) if weight is not None and ctx.needs_input_grad[1] else None
         db = new(C, device=x.device, dtype=torch.float32) if bias is not None and ctx.needs_input_grad[2] else None
         if x.numel() == 0:
-            return dx, dw, db, None, None, None
+            return (dx, *_as_given(dw, db, ctx.types), None, None, None)
         dy = dy.contiguous(memory_format=_channels_last(x))
         code, base, places = _lib.FLOAT_TYPES[x.dtype], stats.data_ptr(), x.shape[2:].numel()
         with _lib.device_of(x) as stream:
@@ -115,7 +124,7 @@ class _GroupNormAct(Function):
                                                                base + 4 * B * ctx.groups, B, places, C, ctx.groups, ctx.act, code,
                                                                ws.data_ptr(), dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), stream),
                        "combo_groupnorm_act_backward")
-        return dx, dw, db, None, None, None
+        return (dx, *_as_given(dw, db, ctx.types), None, None, None)
 
 
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none"):
@@ -148,11 +157,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
         raise ValueError("group_norm_act: more than 2^31 places in a map")
     if not x.is_cuda:
         raise RuntimeError("combo_avs_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
-    if weight is not None:
-        weight = weight.float().contiguous()
-    if bias is not None:
-        bias = bias.float().contiguous()
-    args = (x, weight, bias, int(groups), float(eps), ACTIVATIONS[activation])
+    how = (int(groups), float(eps), ACTIVATIONS[activation])
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _lib.record(_GroupNormAct, *args)
-    return _act_forward(*args)[0]
+        return _lib.record(_GroupNormAct, x, weight, bias, *how)
+    return _act_forward(x, _param(weight), _param(bias), *how)[0]

@@ -42,3 +42,20 @@ def test_capture_beside_a_living_eager_graph_is_refused(name):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(held, want)
+
+
+def test_capture_is_refused_for_norm_parameters_of_the_maps_type():
+    """parameters that the op widens for itself are leaves too"""
+    from combo_avs_amd.ops.groupnorm import group_norm_act
+    m = torch.randn(2, 8, 6, 6, device="cuda").bfloat16().contiguous(memory_format=torch.channels_last)
+    w, b = (torch.rand(8, device="cuda").bfloat16().requires_grad_(True) for _ in range(2))
+    alive = group_norm_act(m, 2, w, b, activation="silu")
+    dw, db = torch.autograd.grad(alive, (w, b), torch.ones_like(alive), retain_graph=True)
+    w32, b32 = (t.detach().float().requires_grad_(True) for t in (w, b))
+    dw32, db32 = torch.autograd.grad(group_norm_act(m, 2, w32, b32, activation="silu"), (w32, b32), torch.ones_like(alive))
+    assert torch.equal(dw, dw32.bfloat16()) and torch.equal(db, db32.bfloat16())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        with torch.cuda.graph(graph):
+            group_norm_act(m, 2, w, b, activation="silu")
