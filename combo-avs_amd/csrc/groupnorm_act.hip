@@ -620,7 +620,7 @@ int run(NormArgs& A, int dtype, int act_, bool back, uintptr_t all, hipStream_t 
 
 // (B * lines bounds every grid: a launch holds less than 2^32 threads)
 bool shape_ok(int B, int HW, int C, int G, int dtype, int act_) {
-  if (B <= 0 || HW <= 0 || C <= 0 || C > kMaxC || G <= 0 || C % G || dtype < 0 || dtype > 2 || act_ < 0 || act_ > 3) return false;
+  if (B <= 0 || HW <= 0 || HW > (1 << 30) || C <= 0 || C > kMaxC || G <= 0 || C % G || dtype < 0 || dtype > 2 || act_ < 0 || act_ > 3) return false;
   const int lines = (C * (dtype == 0 ? 4 : 2) + 127) / 128;
   return (long long)B * C < 0x7fffffffll && B <= (1 << 22) && (long long)B * lines < (1 << 24);
 }

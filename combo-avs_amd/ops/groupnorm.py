@@ -153,8 +153,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
                 raise ValueError(f"group_norm_act: {name} is on {p.device}, x on {x.device}")
     if not x.is_contiguous(memory_format=_channels_last(x)):
         raise ValueError("group_norm_act: x must be channels-last (x.contiguous(memory_format=torch.channels_last), _3d for five dimensions)")
-    if x.shape[2:].numel() >= 1 << 31:
-        raise ValueError("group_norm_act: more than 2^31 places in a map")
+    if x.shape[2:].numel() > 1 << 30:
+        raise ValueError("group_norm_act: more than 2^30 places in a map")
     if not x.is_cuda:
         raise RuntimeError("combo_avs_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
     how = (int(groups), float(eps), ACTIVATIONS[activation])

@@ -48,6 +48,7 @@ def test_entry_points_refuse_bad_arguments_without_a_launch():
     assert all(rc == 1 for rc in (rotary(D=7), rotary(D=2), rotary(D=258), rotary(axes=0), rotary(axes=9), rotary(pos_type=4), rotary(dtype=3),
                                   rotary(B=0), rotary(x=0), rotary(x=4098), rotary(H=1 << 25)))
     assert lib.combo_groupnorm_act_workspace(1, 9, 8, 3, 0, 0) == -1 and lib.combo_groupnorm_act_workspace(1, 9, 4104, 2, 0, 0) == -1
+    assert lib.combo_groupnorm_act_workspace(1, (1 << 30) + 1, 1, 1, 0, 0) == -1 and lib.combo_groupnorm_act_workspace(1, 1 << 30, 1, 1, 0, 0) > 0
     assert lib.combo_groupnorm_act_workspace(1 << 18, 1, 4096, 2, 0, 0) == -1  # more workgroups than a launch holds
     assert lib.combo_groupnorm_act_workspace(2, 9, 8, 2, 0, 0) == 0 and lib.combo_groupnorm_act_workspace(2, 9, 8, 2, 0, 1) == 40
     assert lib.combo_groupnorm_act_workspace(2, 9000, 64, 2, 0, 0) > 0
