@@ -688,8 +688,9 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
   };
   // Delta = o . do carries the rounding of o and of the probabilities that made it, and over few keys that is as large as the rounding of ds.
   // Where this workgroup has the whole row in LDS, delta + sum_j p_j (dp_j - delta) takes its place: the same number without the roundings
-  // (16 keys: dq and dk 1.56 -> 1.44 times the error of one rounding; 77 keys: 1.46, 2048: 1.43).
-  const bool at_hand = keys.lo == 0 && keys.hi == len && steps <= (RW == 4 ? 2 : 1);
+  // (16 keys: dq and dk 1.56 -> 1.42 times the error of one rounding; 60 of which a mask leaves 24: 1.51 -> 1.42; longer walks have 1.43 to 1.47
+  // without it).  It costs a second look at those tiles: 4 x 10 x 4096 rows against 77 keys 29 -> 35 us.
+  const bool at_hand = keys.lo == 0 && keys.hi == len && steps <= F::BUFS;
   auto missing = [&](const T* Kt, const T* Vt, int k0) {
     f32x16 s[KB];
     scores(Kt, s);
@@ -749,12 +750,17 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
       k1.store(kbuf + F::TILE);
       v1.store(vbuf + F::TILE);
     }
+    if (at_hand && steps == 3) {
+      fetch(sk, sv, keys.lo + 2 * F::KT);
+      sk.store(kbuf + 2 * F::TILE);
+      sv.store(vbuf + 2 * F::TILE);
+    }
     __syncthreads();
     if (at_hand) {
-      float sum = missing(kbuf, vbuf, keys.lo);
-      if (steps > 1) {
-        bits.load(words, keys.lo + F::KT, len);
-        sum += missing(kbuf + F::TILE, vbuf + F::TILE, keys.lo + F::KT);
+      float sum = 0.f;
+      for (int t = 0; t < steps; ++t) {
+        if (t) bits.load(words, keys.lo + t * F::KT, len);
+        sum += missing(kbuf + t * F::TILE, vbuf + t * F::TILE, keys.lo + t * F::KT);
       }
       delta += sum;
     }
