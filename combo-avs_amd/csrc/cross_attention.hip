@@ -1239,9 +1239,10 @@ bool desc_ok(const combo_cross_attention_t* d) {
   if (!d || !d->q || !d->k || !d->v || d->B <= 0 || d->Lq <= 0 || d->Lk <= 0 || d->Hq <= 0 || d->Hk <= 0 || d->Hq % d->Hk || d->D <= 0 || d->D > 128 ||
       d->D % 8 || (d->dtype != 1 && d->dtype != 2) || !(d->scale > 0.f) || !std::isfinite(d->scale * 1.4427f))
     return false;
-  if (((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15) return false;
+  if (((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15 || ((uintptr_t)d->kv_lengths | (uintptr_t)d->blocked_bits) & 3) return false;
   for (int i = 0; i < 3; ++i)
-    if ((d->q_stride[i] | d->k_stride[i] | d->v_stride[i]) & 7 || d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0) return false;
+    if ((d->q_stride[i] | d->k_stride[i] | d->v_stride[i]) & 7 || d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0 || d->bits_stride[i] < 0)
+      return false;
   if (d->k_stride[1] > (1 << 22) || d->v_stride[1] > (1 << 22)) return false;  // (32-bit byte offsets inside a tile of 128 keys)
   if ((long long)d->Lq * (d->Hq / d->Hk) >= (1ll << 30) || d->Lk >= (1 << 30)) return false;
   for (const bool back : {false, true}) {  // (workgroups of the largest launches: a grid holds less than 2^32 threads)
@@ -1329,7 +1330,7 @@ long long combo_cross_attention_workspace(const combo_cross_attention_t* d, int 
 }
 
 int combo_cross_attention_forward(const combo_cross_attention_t* d, void* out, float* lse, void* workspace, combo_stream_t stream) {
-  if (!desc_ok(d) || !out || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 31)) return COMBO_EINVAL;
+  if (!desc_ok(d) || !out || ((uintptr_t)out & 15) || ((uintptr_t)lse & 3) || ((uintptr_t)workspace & 31)) return COMBO_EINVAL;
   const Plan p = plan_of(*d, false);
   if (p.splits > 1 && !workspace) return COMBO_EINVAL;
   Args A = args_of(*d);
@@ -1341,7 +1342,7 @@ int combo_cross_attention_forward(const combo_cross_attention_t* d, void* out, f
 int combo_cross_attention_backward(const combo_cross_attention_t* d, const void* out, const float* lse, const void* dout, void* workspace,
                                    void* dq, void* dk, void* dv, combo_stream_t stream) {
   if (!desc_ok(d) || !out || !lse || !dout || !workspace || !dq || (!dk) != (!dv) ||
-      (((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) || ((uintptr_t)workspace & 31))
+      (((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) || ((uintptr_t)lse & 3) || ((uintptr_t)workspace & 31))
     return COMBO_EINVAL;
   const Plan p = plan_of(*d, true);
   Args A = args_of(*d);

@@ -14,6 +14,8 @@
 // Statistics: a thread sums x - K and (x - K)^2 with K its own first value of the channel, in fp32, and hands on (mean, M2); these are
 // joined as M2 = sum M2_i + sum n_i (mean_i - mean)^2.  K is one of the values, so the shift's cancellation is at most n_thread * 2^-24 of M2
 // whatever the offset of the map (a plain sum of squares loses everything once mean^2 > 2^24 var).  All sums have a fixed order.
+#include <initializer_list>
+
 #include "combo_common.h"
 
 namespace {
@@ -625,6 +627,12 @@ bool shape_ok(int B, int HW, int C, int G, int dtype, int act_) {
   return (long long)B * C < 0x7fffffffll && B <= (1 << 22) && (long long)B * lines < (1 << 24);
 }
 
+bool floats_ok(std::initializer_list<const float*> all, const float* workspace) {
+  uintptr_t a = 0;
+  for (const float* p : all) a |= (uintptr_t)p;
+  return !(a & 3) && !((uintptr_t)workspace & 7);  // (the workspace is read in pairs)
+}
+
 }  // namespace
 
 extern "C" {
@@ -644,7 +652,7 @@ int combo_groupnorm_act_forward(const void* x, const float* weight, const float*
   if (!x || (!mean) != (!rstd) || !y || !shape_ok(B, HW, C, G, dtype, act_)) return COMBO_EINVAL;
   if (!workspace && combo_groupnorm_act_workspace(B, HW, C, G, dtype, 0) > 0) return COMBO_EINVAL;
   const uintptr_t all = (uintptr_t)x | (uintptr_t)y;
-  if (all & (dtype == 0 ? 3 : 1)) return COMBO_EINVAL;
+  if (all & (dtype == 0 ? 3 : 1) || !floats_ok({weight, bias, mean, rstd}, workspace)) return COMBO_EINVAL;
   NormArgs A = {};
   A.x = x, A.w = weight, A.bias = bias, A.mean = mean, A.rstd = rstd, A.part = workspace, A.out = y, A.eps = eps;
   A.B = B, A.HW = HW, A.C = C, A.G = G, A.per = C / G;
@@ -656,7 +664,7 @@ int combo_groupnorm_act_backward(const void* dy, const void* x, const float* wei
                                  combo_stream_t stream) {
   if (!dy || !x || !mean || !rstd || !workspace || !dx || !shape_ok(B, HW, C, G, dtype, act_)) return COMBO_EINVAL;
   const uintptr_t all = (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx;
-  if (all & (dtype == 0 ? 3 : 1)) return COMBO_EINVAL;
+  if (all & (dtype == 0 ? 3 : 1) || !floats_ok({weight, bias, mean, rstd, dweight, dbias}, workspace)) return COMBO_EINVAL;
   NormArgs A = {};
   A.x = x, A.dy = dy, A.w = weight, A.bias = bias, A.mean = const_cast<float*>(mean), A.rstd = const_cast<float*>(rstd), A.part = workspace;
   A.out = dx, A.dw = dweight, A.db = dbias;

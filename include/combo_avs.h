@@ -698,7 +698,8 @@ int combo_cross_attention_pack(const unsigned char* blocked, long long stride_b,
  *   y = act((x - mean) rstd weight + bias), act 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf); x, y, dy, dx of `dtype` (0 fp32, 1 bf16, 2 fp16),
  *   weight / bias fp32 (NULL: 1 / 0).  mean, rstd [B,G]: written by the forward pass (NULL: not
  *   wanted), read by the backward pass.
- *   workspace: combo_groupnorm_act_workspace floats (-1: shape refused, 0: none needed), not shared by calls that may run at the same time.
+ *   workspace: combo_groupnorm_act_workspace floats, 8-byte aligned (-1: shape refused, 0: none needed), not shared by calls that may run at
+ *   the same time.
  *   dweight, dbias [C] fp32 (NULL: not wanted).  All sums in a fixed order.
  * ---------------------------------------------------------------------------------------------- */
 long long combo_groupnorm_act_workspace(int B, int HW, int C, int G, int dtype, int backward_pass);

@@ -102,3 +102,21 @@ def test_cross_attention_entry_points_refuse_without_a_launch():
     assert lib.combo_cross_attention_forward(desc(Lk=1000), one, 0, 0, 0) == 1  # split keys need their workspace
     assert lib.combo_cross_attention_backward(desc(), one, one, one, one, one, one, 0, 0) == 1  # dk without dv
     assert lib.combo_cross_attention_pack(one, 1, 1, 1, 1, 0, 1, 1, 1, one, 0) == 1
+
+
+def test_entry_points_refuse_misaligned_side_tensors():
+    from combo_avs_amd import _lib
+    from combo_avs_amd.ops.cross_attention import _DESC
+    lib, one = _lib.lib(), 4096  # (never dereferenced: every call below is refused on the host)
+    for w, b, ws, mean, rstd in ((one + 2, 0, one, one, one), (0, one + 1, one, one, one), (0, 0, one + 4, one, one), (0, 0, one, one + 2, one), (0, 0, one, one, one + 2)):
+        assert lib.combo_groupnorm_act_forward(one, w, b, 2, 9000, 64, 2, 1e-5, 0, 0, ws, mean, rstd, one, 0) == 1
+        assert lib.combo_groupnorm_act_backward(one, one, w, b, mean, rstd, 2, 9000, 64, 2, 0, 0, ws, one, one, one, 0) == 1
+    assert lib.combo_groupnorm_act_backward(one, one, 0, 0, one, one, 2, 9000, 64, 2, 0, 0, one, one, one + 2, one, 0) == 1
+
+    def desc(lengths=0, bits=0, bit_stride=0):
+        return _DESC.pack(one, one, one, *(64, 32, 16) * 3, lengths, bits, bit_stride, 0, 0, 1, 2, 3, 2, 1, 16, 1, 0.25)
+    for bad in (desc(lengths=one + 2), desc(bits=one + 2), desc(bits=one, bit_stride=-1)):
+        assert lib.combo_cross_attention_workspace(bad, 0) == -1
+        assert lib.combo_cross_attention_forward(bad, one, 0, one, 0) == 1
+    assert lib.combo_cross_attention_forward(desc(), one, one + 2, one, 0) == 1
+    assert lib.combo_cross_attention_backward(desc(), one, one + 2, one, one, one, one, one, 0) == 1
