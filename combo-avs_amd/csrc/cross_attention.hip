@@ -233,7 +233,7 @@ __device__ __forceinline__ Range split_range(int len, int splits, int s, int til
 // ---- forward ------------------------------------------------------------------------------------------------------------------
 
 // few rows, in blocks of 32: the four waves hold the same rows and share the keys of a tile, 32 each.  Bound by the read of K and V: 16 x 8 x 16384
-// keys of 128 (1.07 GB) 198 us = 5.4 TB/s, ragged lengths 153; a single round of workgroups (4 x 8 x 784 of 32) 8 us, which are latency.
+// keys of 128 (1.07 GB) 198 us = 5.4 TB/s, ragged lengths 153; a single round of workgroups (4 x 8 x 784 of 32) 9 us, which are latency.
 template <int DP>
 struct Few {
   static constexpr int KW = 4, KT = 32 * KW, TILE = KT * Tile<DP>::PITCH;
@@ -1193,8 +1193,8 @@ struct Plan {
 
 // Splits of the other axis when there are few workgroups: as many as `slots`, one round of what the chip holds, allow (4 x 10 x 4096 rows against 77
 // keys: dk, dv in 13 shares are 520 workgroups and take 26.2 us, in 12 21.8; 3 x 8 x 300 rows over 5000 keys of 128: 24 shares 49.0, 21 38.9).
-// Left whole are a walk of a few tiles, which costs no more than the join and saves a launch (8 x 100 rows over 256 keys of 64: 7.5 against 9.7 us
-// replayed, 13.8 against 17.3 called; one row of 4 x 8 over 784 keys of 32: 8.6 against 9.6, 14.2 against 18.2; replayed, 8 tiles of 64: 10.8
+// Left whole are a walk of a few tiles, which costs no more than the join and saves a launch (8 x 100 rows over 256 keys of 64: 6.1 against 9.7 us
+// replayed, 13.6 against 17.3 called; one row of 4 x 8 over 784 keys of 32: 9.1 against 9.6, 13.9 against 18.2; replayed, 8 tiles of 64: 10.8
 // against 10.3, 8 of 128: 16.6 against 11.3), and from one workgroup a CU on a short axis: 320 workgroups of 13 tiles take 26.8 us, and in two
 // halves 22.7 us and a join of 4.2 us and one more launch.
 int pick_splits(long long groups, int tiles, int D, int slots) {
@@ -1207,15 +1207,15 @@ int pick_splits(long long groups, int tiles, int D, int slots) {
 
 // Blocks of 128 rows read a key once for all of them; blocks of 32 are four times as many.  So these are taken for 32 rows, and where 128 would
 // leave CUs idle or need a join and 32 need none (forward, dq, each with its join, 128 against 32 rows a block): 8 x 8 x 100 rows over 784 keys of 32
-// 14.4, 14.9 against 10.1, 10.5 us; 16 x 8 x 100 over 784 of 64 19.9, 22.7 against 15.6, 18.2; 2 x 8 x 512 over 1024 of 128 26.8, 30.3 against
-// 18.5, 22.9; 1 x 8 x 1024 over 2048 of 128 32.8, 36.3 against 30.9, 35.9.  Not for dq of more than 64 dimensions, with one workgroup a CU, beyond
-// one round of them: 16 x 8 x 100 over 784 of 128 32.0 against 40.4.  Longer walks stay with 128: 1 x 8 x 1024 over 8192 of 128 62.4, 72.2
-// against 93.5, 158.
+// 14.2, 15.0 against 10.7, 12.0 us; 1 x 8 x 1024 over 1500 of 64 23.9, 22.3 against 18.2, 20.6; 2 x 8 x 512 over 1024 of 128 27.5, 30.5 against 20.9,
+// 27.8; even at 1 x 8 x 1000 over 2000 of 32 (16.8, 19.0 against 18.0, 19.0, and a launch less) and 1 x 8 x 1024 over 2048 of 128 (35.1, 36.2
+// against 35.7, 41.8), and longer walks stay with 128.  Not for dq of more than 64 dimensions, with one workgroup a CU, beyond one round of them:
+// 16 x 8 x 100 over 784 of 128 32.0 against 40.4.
 Plan plan_of(const combo_cross_attention_t& d, bool back) {
   Plan p;
   const int G = d.Hq / d.Hk;
   const long long rows = (long long)d.Lq * G, bh = (long long)d.B * d.Hk, small = bh * ((rows + 31) / 32);
-  const bool whole = bh * ((rows + 127) / 128) < 256 && d.Lk <= 2048 && pick_splits(small, (d.Lk + 127) / 128, d.D, 512) == 1 &&
+  const bool whole = bh * ((rows + 127) / 128) < 256 && d.Lk <= (d.D > 64 ? 1024 : 2048) && pick_splits(small, (d.Lk + 127) / 128, d.D, 512) == 1 &&
                      !(back && d.D > 64 && small > 256);
   p.rows = rows <= 32 || whole ? 32 : 128;
   p.tiles = (int)((rows + p.rows - 1) / p.rows);
@@ -1241,7 +1241,8 @@ bool desc_ok(const combo_cross_attention_t* d) {
     return false;
   if (((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15 || ((uintptr_t)d->kv_lengths | (uintptr_t)d->blocked_bits) & 3) return false;
   for (int i = 0; i < 3; ++i)
-    if ((d->q_stride[i] | d->k_stride[i] | d->v_stride[i]) & 7 || d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0 || d->bits_stride[i] < 0)
+    if ((d->q_stride[i] | d->k_stride[i] | d->v_stride[i]) & 7 || d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0 ||
+        d->bits_stride[i] < 0)
       return false;
   if (d->k_stride[1] > (1 << 22) || d->v_stride[1] > (1 << 22)) return false;  // (32-bit byte offsets inside a tile of 128 keys)
   if ((long long)d->Lq * (d->Hq / d->Hk) >= (1ll << 30) || d->Lk >= (1 << 30)) return false;
