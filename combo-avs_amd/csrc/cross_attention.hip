@@ -872,6 +872,10 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
   const T* q = reinterpret_cast<const T*>(A.q) + b * A.qb;
   const T* g = static_cast<const T*>(A.dout);
   const long long side = ((long long)b * A.Hk + hk) * A.rows;
+  // fp16 holds p as 2^12 p: over thousands of keys most of p is under 2^-14, where the type runs out of digits (16384 keys: dv 1.55 -> 1.42 times
+  // the error of one rounding); p <= 1 stays in range.  So lse comes 12 less, delta and dp 2^-12 times, and dv ends with the reverse.
+  constexpr bool half_type = std::is_same_v<T, _Float16>;
+  constexpr float kDown = half_type ? 1.f / 4096.f : 1.f;
   // a thread's vectors of a tile, of Q and of dO by turns (one vector: half of the threads each); where G divides a tile's rows they move on by the
   // same distance from tile to tile
   constexpr int N = 2 * F::RT * (DP / 8) / 256, STEP = 256 / (DP / 8);
@@ -909,7 +913,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
       const int r = rt * F::RT + threadIdx.x % F::RT;
       const float* from = threadIdx.x < F::RT ? A.lse : A.delta;
       rl = r < A.rows ? from[side + r] : (threadIdx.x < F::RT ? kInf : 0.f);
-      if (std::is_same_v<T, _Float16> && threadIdx.x < F::RT) rl -= 12.f;  // (below)
+      if constexpr (half_type) rl = threadIdx.x < F::RT ? rl - 12.f : rl * kDown;
     }
     if (A.bits) {
       const int x = threadIdx.x, r = rt * F::RT + x % F::RT, w = tile * 4 + x / F::RT;
@@ -972,10 +976,6 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
 #pragma unroll
       for (int d = 0; d < NT; ++d) o[d] = Type<T>::mfma(x[st][d], y[st], o[d]);
   };
-  // fp16 holds p as 2^12 p: over thousands of keys most of p is under 2^-14, where the type runs out of digits (16384 keys: dv 1.55 -> 1.41 times
-  // the error of one rounding); p <= 1 stays in range.  lse is read 12 less, dv ends with the reverse.
-  constexpr bool half_type = std::is_same_v<T, _Float16>;
-  constexpr float kUp = half_type ? 4096.f : 1.f, kDown = 1.f / kUp;
   // a value per row (lse or delta) for this lane's 16 rows
   auto read_side = [&](const float* side_, f32x16& x) {
 #pragma unroll
@@ -1019,7 +1019,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
       over_rows(next, k, s);
       read_cols(g_tile(bt), cols);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= half_type ? (dp[i] - L[i]) * kDown : dp[i] - L[i];
+      for (int i = 0; i < 16; ++i) x[i] *= fmaf(dp[i], kDown, -L[i]);
       ds[0] = pack<T>(x, 0);
       ds[1] = pack<T>(x, 1);
       __builtin_amdgcn_sched_barrier(0);
