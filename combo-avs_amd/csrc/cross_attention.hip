@@ -119,6 +119,36 @@ __device__ __forceinline__ float both_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// fp16 holds 30 binades, and a score gradient ds = p (dp - delta) carries the size of a probability (1 / keys) times that of the upstream gradient:
+// rounded as it is, ds of 16384 keys under upstream gradients of 2^-10 lay below 2^-24, and dq was off by 16 times its own rounding.  So a lane holds
+// its row (dq) or key (dk) of ds, and its accumulators, at 2^up and takes that out again at the end.  `up` starts high and only falls: where a value of
+// a tile reaches 2, the lane's largest is brought into [2^-7, 2^-6) and the accumulators follow, at the first tile and a few times at most behind it.
+// What then lies under 2^-14 is rounded by at most 2^-25, 1/64 of the largest's own rounding, and ds past 65504 stay in range.  bf16 has fp32's
+// exponents and holds ds as it is.  Cost in fp16: 4 x 16 x 4096 x 4096 x 128, training, 3035 -> 3254 us; 4 x 10 x 4096 rows against 77 keys 85 -> 87.
+struct Held {
+  float up = 60.f;
+  static __device__ __forceinline__ float power(float e) { return __builtin_amdgcn_ldexpf(1.f, (int)e); }
+  // top: this lane's largest |x| -> the factor that x and the accumulators of its row or key, which two lanes share, take now (1 where in range)
+  __device__ __forceinline__ float lower(float top) {
+    top = other_max(top);
+    if (!(top >= 2.f)) return 1.f;
+    const float fall = (float)(__builtin_amdgcn_frexp_expf(top) + 6);
+    up -= fall;
+    return power(-fall);
+  }
+};
+// nonzero: one of 16 packed values is 2 or more (bit 14 of fp16, its highest exponent bit; Inf and NaN have it too)
+template <typename X8>
+__device__ __forceinline__ unsigned two_or_more(const X8& a, const X8& b) {
+  const u32x4 x = __builtin_bit_cast(u32x4, a), y = __builtin_bit_cast(u32x4, b);
+  return (x[0] | x[1] | x[2] | x[3] | y[0] | y[1] | y[2] | y[3]) & 0x40004000u;
+}
+__device__ __forceinline__ float largest(const f32x16& x, float top) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, fabsf(x[i])), fabsf(x[i + 1]));
+  return top;
+}
+
 // index of register i of a 32 x 32 result along its rows
 __device__ __forceinline__ int reg_row(int i, int half) { return 8 * (i >> 2) + 4 * half + (i & 3); }
 
@@ -668,22 +698,55 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
   // and is now at 1.05 (40 x 8 x 100 rows over 784 keys of 32: 28 -> 33 us, 16 x 8 x 4 rows over 16384 of 128: 188 -> 196).
   constexpr int PIECES = DP == 32 || RW == 1 ? 2 : 1;
   typedef x8 Grad[KB][2][PIECES];
-  auto gradient = [&](const T* Vt, const f32x16 (&s)[KB], Grad& ds) {
+  constexpr bool kHeld = std::is_same_v<T, _Float16>;
+  Held hold;
+  float base = kHeld ? lse - hold.up : lse;  // (p comes at 2^up)
+  auto gradient = [&](const T* Vt, const f32x16 (&s)[KB], f32x16 (&x)[KB]) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       f32x16 dp;
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) dp = Type<T>::mfma(operand<T, DP>(Vt, (kw * KB + kb) * 32, d), g[d], d ? dp : zero16());
-      f32x16 x;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], A.c, -lse));
+      for (int i = 0; i < 16; ++i) x[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], A.c, -base));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= dp[i] - delta;
+      for (int i = 0; i < 16; ++i) x[kb][i] *= dp[i] - delta;
+    }
+  };
+  auto round_off = [&](f32x16 (&x)[KB], Grad& ds) {
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        ds[kb][st][0] = pack<T>(x, st);
-        if constexpr (PIECES == 2) ds[kb][st][1] = left_off<T>(x, st, ds[kb][st][0]);
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) ds[kb][st][0] = pack<T>(x[kb], st);
+    if constexpr (kHeld) {
+      unsigned large = 0u;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) large |= two_or_more(ds[kb][0][0], ds[kb][1][0]);
+      if (__any(large)) {
+        float top = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) top = largest(x[kb], top);
+        const float f = hold.lower(top);
+        base = lse - hold.up;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[kb][i] *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int st = 0; st < 2; ++st) ds[kb][st][0] = pack<T>(x[kb], st);
       }
+    }
+    if constexpr (PIECES == 2) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int st = 0; st < 2; ++st) ds[kb][st][1] = left_off<T>(x[kb], st, ds[kb][st][0]);
     }
   };
   // Delta = o . do carries the rounding of o and of the probabilities that made it, and over few keys that is as large as the rounding of ds.
@@ -736,11 +799,12 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
 #pragma unroll
         for (int w = 0; w < F::KW; ++w) delta += sums[w * 32 + (lane & 31)];
       }
-      f32x16 s[KB];
+      f32x16 s[KB], x[KB];
       Grad ds;
       scores(kbuf, s);
       mask(k0, s);
-      gradient(vbuf, s, ds);
+      gradient(vbuf, s, x);
+      round_off(x, ds);
       add_keys(kbuf, ds);
     }
   } else if (steps > 0) {
@@ -772,15 +836,25 @@ __global__ void __launch_bounds__(256, RW == 1 && DP == 128 ? 1 : 2) cross_dq_ke
       if (t + 2 < steps) fetch(sk, sv, k0 + 2 * F::KT);
       __syncthreads();
       mask(k0, s);
+      f32x16 x[KB];
       Grad ds;
-      gradient(vbuf + kt, s, ds);
-      scores(kbuf + kn, s);  // (behind the last tile: what lies in the buffer, not used)
+      gradient(vbuf + kt, s, x);
+      if constexpr (kHeld) scores(kbuf + kn, s);  // (ahead of the branch in round_off, so that they share a basic block with the gradient)
+      round_off(x, ds);
+      if constexpr (!kHeld) scores(kbuf + kn, s);  // (behind the last tile: what lies in the buffer, not used)
       add_keys(kbuf + kt, ds);
       sk.store(kbuf + kf);  // tile t + 2 (none left: what was there, not used)
       sv.store(vbuf + kf);
-      const int x = kt;
-      kt = kn, kn = kf, kf = x;
+      const int y = kt;
+      kt = kn, kn = kf, kf = y;
     }
+  }
+  if constexpr (kHeld) {
+    const float back = Held::power(-hold.up);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] *= back;
   }
   if (on && half == 0 && kw == 0 && split == 0) A.delta[at] = delta;
   auto store = [&](int d, const float (&x)[4]) {
@@ -873,9 +947,11 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
   const T* g = static_cast<const T*>(A.dout);
   const long long side = ((long long)b * A.Hk + hk) * A.rows;
   // fp16 holds p as 2^12 p: over thousands of keys most of p is under 2^-14, where the type runs out of digits (16384 keys: dv 1.55 -> 1.42 times
-  // the error of one rounding); p <= 1 stays in range.  So lse comes 12 less, delta and dp 2^-12 times, and dv ends with the reverse.
+  // the error of one rounding); p <= 1 stays in range.  So lse comes 12 less and dv ends with the reverse; ds has a scale of its own (Held).
   constexpr bool half_type = std::is_same_v<T, _Float16>;
   constexpr float kDown = half_type ? 1.f / 4096.f : 1.f;
+  Held hold;
+  float lift = Held::power(hold.up - 12.f);
   // a thread's vectors of a tile, of Q and of dO by turns (one vector: half of the threads each); where G divides a tile's rows they move on by the
   // same distance from tile to tile
   constexpr int N = 2 * F::RT * (DP / 8) / 256, STEP = 256 / (DP / 8);
@@ -913,7 +989,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
       const int r = rt * F::RT + threadIdx.x % F::RT;
       const float* from = threadIdx.x < F::RT ? A.lse : A.delta;
       rl = r < A.rows ? from[side + r] : (threadIdx.x < F::RT ? kInf : 0.f);
-      if constexpr (half_type) rl = threadIdx.x < F::RT ? rl - 12.f : rl * kDown;
+      if constexpr (half_type) rl = threadIdx.x < F::RT ? rl - 12.f : rl;
     }
     if (A.bits) {
       const int x = threadIdx.x, r = rt * F::RT + x % F::RT, w = tile * 4 + x / F::RT;
@@ -985,6 +1061,32 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
     }
   };
   auto lse_of = [&](int buf) { return reinterpret_cast<const float*>(lds + buf + F::TILE); };
+  // ds to its scale (fp16) and type.  With one wave a SIMD the scale, the check and the branch stand beside the products of dV, where the vector unit is
+  // free (64 x 4096 x 4096 x 128: 2180 -> 2030 us; ds without a scale 1910); at 32 dimensions x would live longer than three workgroups a CU
+  // have registers for (40 x 8 x 100 rows and 784 keys, the whole pass: 70.5 against 76.7).
+  constexpr bool kLate = half_type && DP == 128;
+  auto round_off = [&](f32x16& x, x8 (&ds)[2]) {
+    if constexpr (half_type) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= lift;
+    }
+    ds[0] = pack<T>(x, 0);
+    ds[1] = pack<T>(x, 1);
+    if constexpr (half_type) {
+      if (__any(two_or_more(ds[0], ds[1]))) {
+        const float f = hold.lower(largest(x, 0.f));
+        lift *= f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= f;
+#pragma unroll
+        for (int d = 0; d < NT; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ak[d][i] *= f;
+        ds[0] = pack<T>(x, 0);
+        ds[1] = pack<T>(x, 1);
+      }
+    }
+  };
   if (lo < hi) {
     fetch(lo);
     park(lds);
@@ -1019,12 +1121,12 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
       over_rows(next, k, s);
       read_cols(g_tile(bt), cols);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= fmaf(dp[i], kDown, -L[i]);
-      ds[0] = pack<T>(x, 0);
-      ds[1] = pack<T>(x, 1);
+      for (int i = 0; i < 16; ++i) x[i] *= dp[i] - L[i];
+      if constexpr (!kLate) round_off(x, ds);
       __builtin_amdgcn_sched_barrier(0);
       over_cols(cols, p, av);
       read_cols(q_tile(bt), cols2);
+      if constexpr (kLate) round_off(x, ds);
       __builtin_amdgcn_sched_barrier(0);
       over_cols(cols2, ds, ak);
       read_rows(g_tile(bn), rows);
@@ -1033,6 +1135,13 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) cross_dkv_kernel(const
       const int y = bt;
       bt = bn, bn = bf, bf = y;
     }
+  }
+  if constexpr (half_type) {
+    const float back = Held::power(-hold.up);
+#pragma unroll
+    for (int d = 0; d < NT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ak[d][i] *= back;
   }
   if (key >= A.Lk) return;
   if (!open) {  // keys behind the length or blocked for all: zeros

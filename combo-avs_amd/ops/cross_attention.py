@@ -106,8 +106,8 @@ def cross_attention(q, k, v, kv_lengths=None, blocked=None, scale=None):
     gradient.  States behind a sample's length, and states that a mask shared by all queries and heads blocks, may hold anything; a state
     that only some queries are kept from has to be finite.  scale: positive, D ** -0.5 by default.  Probabilities enter the
     second product in the tensors' type (in two pieces where few rows make the matrix work cheap), as do the score gradients in the
-    backward pass; sums, statistics and gradients accumulate in fp32 in a fixed order (runs repeat bit for bit); in fp16 a score
-    gradient beyond 65504 overflows."""
+    backward pass, in fp16 at a scale per query and per key that keeps their digits for upstream gradients of any size; sums, statistics and
+    gradients accumulate in fp32 in a fixed order (runs repeat bit for bit)."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"cross_attention: q [B, Lq, Hq, D], k and v [B, Lk, Hk, D]: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     B, Lq, Hq, D = q.shape
