@@ -8,6 +8,7 @@ import os
 import weakref
 
 import torch as _torch
+import torch.autograd.forward_ad as _forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libcombo_avs_hip.so")
@@ -205,6 +206,15 @@ def current_stream():
 
 
 
+def recorded(*tensors):
+    """Whether a call has to go through its autograd Function: one of the tensors wants a gradient, or forward-mode derivatives or a trace are being
+    taken - there the Function says that it has no tangent, or enters the traced graph, where a bare launch on the tensors' memory would leave a
+    result without its tangent and a trace without the call."""
+    if _torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return _forward_ad._current_level >= 0 or _torch._C._get_tracing_state() is not None
+
+
 _eager_graphs = weakref.WeakKeyDictionary()  # {autograd node recorded on the default stream: its leaves (weak)}
 
 
@@ -221,7 +231,7 @@ def record(function, *args):
                                "alive: drop its outputs (or detach them) before the capture, or record them on another stream")
         return function.apply(*args)
     out = function.apply(*args)
-    if _raw_stream(_current_device()) == 0:
+    if out.grad_fn is not None and _raw_stream(_current_device()) == 0:
         leaves = [weakref.ref(t) for t in args if torch.is_tensor(t) and t.requires_grad and t.is_leaf]
         if leaves:
             _eager_graphs[out.grad_fn] = leaves

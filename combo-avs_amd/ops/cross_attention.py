@@ -118,7 +118,7 @@ def cross_attention(q, k, v, kv_lengths=None, blocked=None, scale=None):
         raise ValueError(f"cross_attention: head dimension {D}: a multiple of 8, at most {MAX_HEAD_DIM}")
     if Hk < 1 or Hq % Hk:
         raise ValueError(f"cross_attention: {Hq} query heads on {Hk} key heads")
-    scale = D ** -0.5 if scale is None else float(scale)
+    scale = float(D ** -0.5 if scale is None else scale)
     if not 1e-37 < scale < 2e38:
         raise ValueError(f"cross_attention: scale {scale}: positive and finite in fp32")
     if kv_lengths is not None:
@@ -140,7 +140,7 @@ def cross_attention(q, k, v, kv_lengths=None, blocked=None, scale=None):
         if kv_lengths.dtype == torch.int64:
             kv_lengths = kv_lengths.clamp(0, Lk).to(torch.int32)
         kv_lengths = kv_lengths.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _lib.recorded(q, k, v):
         return _lib.record(_CrossAttention, q, k, v, kv_lengths, blocked, scale)
     if q.numel() == 0 or k.numel() == 0:
         return torch.zeros(q.shape, device=q.device, dtype=q.dtype)

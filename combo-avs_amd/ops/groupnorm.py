@@ -74,7 +74,7 @@ def _act_workspace(x, places, groups, code, backward):
 
 def _act_forward(x, weight, bias, groups, eps, act, keep=False):
     """weight, bias: contiguous fp32 or None -> (y, mean and rstd [2, B, groups] for the backward pass or None)"""
-    B, C, places = x.shape[0], x.shape[1], x.shape[2:].numel()
+    B, C, places = int(x.shape[0]), int(x.shape[1]), x.shape[2:].numel()
     y = torch.empty_like(x)  # (preserves channels_last)
     stats = torch.empty(2, B, groups, device=x.device, dtype=torch.float32) if keep else None
     if x.numel() == 0:
@@ -158,6 +158,6 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
     if not x.is_cuda:
         raise RuntimeError("combo_avs_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
     how = (int(groups), float(eps), ACTIVATIONS[activation])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _lib.recorded(x, weight, bias):
         return _lib.record(_GroupNormAct, x, weight, bias, *how)
     return _act_forward(x, _param(weight), _param(bias), *how)[0]

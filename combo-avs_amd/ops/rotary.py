@@ -88,7 +88,7 @@ def rotary_axes(x, positions, sections, base=10000.0, interleaved=False, shared_
     if not (x.is_cuda and positions.is_cuda):
         raise RuntimeError("combo_avs_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
     how = (sections, base, bool(interleaved), bool(shared_ladder))
-    if x.requires_grad and torch.is_grad_enabled():
+    if _lib.recorded(x, positions):
         return _lib.record(_Rotary, x, positions, how)
     return _rotate(x, positions, *how, False)
 
