@@ -192,6 +192,7 @@ FLOAT_TYPES = {_torch.float32: 0, _torch.bfloat16: 1, _torch.float16: 2}  # dtyp
 # small launch's 14 (a torch built without GPU support has neither function; nothing is launched there)
 _current_device = getattr(_torch._C, "_cuda_getDevice", None) or (lambda: _torch.cuda.current_device())
 _raw_stream = getattr(_torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: _torch.cuda.current_stream(index).cuda_stream)
+_grad_enabled, _tracing = _torch.is_grad_enabled, _torch._C._get_tracing_state
 
 
 def ptr(t):
@@ -210,9 +211,13 @@ def recorded(*tensors):
     """Whether a call has to go through its autograd Function: one of the tensors wants a gradient, or forward-mode derivatives or a trace are being
     taken - there the Function says that it has no tangent, or enters the traced graph, where a bare launch on the tensors' memory would leave a
     result without its tangent and a trace without the call."""
-    if _torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if _forward_ad._current_level >= 0 or _tracing() is not None:
         return True
-    return _forward_ad._current_level >= 0 or _torch._C._get_tracing_state() is not None
+    if _grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 _eager_graphs = weakref.WeakKeyDictionary()  # {autograd node recorded on the default stream: its leaves (weak)}
