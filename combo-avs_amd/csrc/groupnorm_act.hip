@@ -28,43 +28,71 @@ enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec { T v[V]; };
 
-// 1 / x to one unit in the last place (v_rcp_f32): a full division is ten instructions, and an activation map is short of them - SiLU by
-// division took 39 us for a 64 MB bf16 map, half of it in the vector unit
+// 1 / x to one unit in the last place (v_rcp_f32): a full division is ten instructions, and a 16-bit activation map is short of them - SiLU by
+// division took 39 us for a 64 MB bf16 map, half of it in the vector unit.  fp32 maps move twice the bytes and take the full functions.
 __device__ __forceinline__ float quick_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
-__device__ __forceinline__ float sigmoid(float z) { return quick_rcp(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z)); }
-// the normal distribution function by erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x) (Abramowitz and Stegun 7.1.26, error under 1.5e-7):
-// the small side keeps its relative size, and the exponential is the one of the density below
-__device__ __forceinline__ float normal_cdf(float z, float& density) {
-  const float x = fabsf(z) * 0.70710678f, t = quick_rcp(fmaf(0.3275911f, x, 1.f)), e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
-  float q = fmaf(t, 1.061405429f, -1.453152027f);
-  q = fmaf(t, q, 1.421413741f);
-  q = fmaf(t, q, -0.284496736f);
-  q = fmaf(t, q, 0.254829592f);
-  const float tail = 0.5f * q * t * e;
-  density = 0.39894228f * e;
-  return z < 0.f ? tail : 1.f - tail;
+template <bool FULL>
+__device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (FULL) return 1.f / (1.f + expf(-z));
+  return quick_rcp(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z));
 }
 
-template <int ACT>
+template <int N>
+__device__ __forceinline__ float polynomial(const float (&c)[N], float x) {
+  float y = c[N - 1];
+#pragma unroll
+  for (int i = N - 2; i >= 0; --i) y = fmaf(x, y, c[i]);
+  return y;
+}
+
+// The normal distribution function and its density d(z).  With a = |z| the tail is R(a) exp(-a^2 / 2), and R, which falls from 1 / 2 like
+// 1 / (a sqrt(2 pi)), is t (c0 + c1 t + ..) in t = 1 / (1 + s a): coefficients fitted here for the smallest relative error (weighted least squares over
+// a of 0 to 14.5), so the small side keeps its relative size.  16-bit maps: six terms, 4.6e-6 of the tail, 1 / 50 of half a step of fp16.  fp32 maps:
+// seven terms from a = 1 on (7e-8), below that 1 / 2 + z P(z^2) with P fitted likewise (7e-10), and the exponent in two pieces (its rounding alone would be
+// 1.4e-6 at z = -6): 7 u of either side, u = 2^-24, root mean square of GELU over a normal z 2.3e-8.
+template <bool FULL>
+__device__ __forceinline__ float normal_cdf(float z, float& density) {
+  if constexpr (FULL) {
+    constexpr float kTail[7] = {0.11167358f, 0.11232360f, 0.09767063f, 0.10959552f, -0.0027825537f, 0.13058622f, -0.059144225f};
+    constexpr float kCentre[6] = {0.39894229f, -0.06649036f, 0.009973324f, -0.0011863301f, 1.1348650e-4f, -7.6542565e-6f};
+    const float a = fminf(fabsf(z), 15.f);  // (exp(-15^2 / 2) is 0 here, and 15^2 has a finite square's error below)
+    const float h = a * a, l = fmaf(a, a, -h), x = -0.72134752f * h;
+    const float rest = fmaf(h, -0.72134752f, -x) + fmaf(h, -9.6298149e-9f, -0.72134752f * l);
+    const float e0 = __builtin_amdgcn_exp2f(x), e = fmaf(0.69314718f * e0, rest, e0);
+    density = 0.39894228f * e;
+    if (a < 1.f) return fmaf(z, polynomial(kCentre, h), 0.5f);
+    const float t = 1.f / fmaf(0.28f, a, 1.f), tail = polynomial(kTail, t) * t * e;
+    return z < 0.f ? tail : 1.f - tail;
+  } else {
+    constexpr float kTail[6] = {0.12386069f, 0.12044134f, 0.13342951f, 0.015745264f, 0.18044983f, -0.073928952f};
+    const float t = quick_rcp(fmaf(0.31f, fabsf(z), 1.f)), e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+    density = 0.39894228f * e;
+    const float tail = polynomial(kTail, t) * t * e;
+    return z < 0.f ? tail : 1.f - tail;
+  }
+}
+
+// FULL: to the last digits of fp32; else to what a 16-bit result shows of them
+template <int ACT, bool FULL>
 __device__ __forceinline__ float act(float z) {
   if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;  // (a NaN stays one)
-  if constexpr (ACT == ACT_SILU) return z * sigmoid(z);
+  if constexpr (ACT == ACT_SILU) return z * sigmoid<FULL>(z);
   if constexpr (ACT == ACT_GELU) {
     float d;
-    return z * normal_cdf(z, d);
+    return z * normal_cdf<FULL>(z, d);
   }
   return z;
 }
-template <int ACT>
+template <int ACT, bool FULL>
 __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (ACT == ACT_SILU) {
-    const float s = sigmoid(z);
+    const float s = sigmoid<FULL>(z);
     return s * fmaf(z, 1.f - s, 1.f);
   }
   if constexpr (ACT == ACT_GELU) {
     float d;
-    const float c = normal_cdf(z, d);
+    const float c = normal_cdf<FULL>(z, d);
     return fmaf(z, d, c);
   }
   return 1.f;
@@ -256,7 +284,7 @@ __device__ __forceinline__ void apply_tokens(const NormArgs& A, int b, int c0, i
       const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + off);
       Vec<T, V> o;
 #pragma unroll
-      for (int k = 0; k < V; ++k) o.v[k] = (T)act<ACT>(fmaf((float)v.v[k] - m[k], a[k], bb[k]));
+      for (int k = 0; k < V; ++k) o.v[k] = (T)act<ACT, sizeof(T) == 4>(fmaf((float)v.v[k] - m[k], a[k], bb[k]));
       *reinterpret_cast<Vec<T, V>*>(y + off) = o;
     }
   }
@@ -353,7 +381,7 @@ __device__ __forceinline__ void channel_grads(const NormArgs& A, int b, int c0, 
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const float xh = ((float)xv.v[k] - m[k]) * r[k];
-        const float dz = (float)gv.v[k] * act_slope<ACT>(fmaf(xh, w[k], bb[k]));
+        const float dz = (float)gv.v[k] * act_slope<ACT, sizeof(T) == 4>(fmaf(xh, w[k], bb[k]));
         u[k] += dz;
         v[k] = fmaf(dz, xh, v[k]);
       }
@@ -429,7 +457,7 @@ __device__ __forceinline__ void dx_tokens(const NormArgs& A, int b, int c0, int 
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const float xh = ((float)xv.v[k] - m[k]) * r[k];
-        const float dz = (float)gv.v[k] * act_slope<ACT>(fmaf(xh, w[k], bb[k]));
+        const float dz = (float)gv.v[k] * act_slope<ACT, sizeof(T) == 4>(fmaf(xh, w[k], bb[k]));
         o.v[k] = (T)(r[k] * fmaf(-xh, a2[k], fmaf(dz, w[k], -a1[k])));
       }
       *reinterpret_cast<Vec<T, V>*>(dx + off) = o;
