@@ -45,12 +45,12 @@ __device__ __forceinline__ double position(const RotaryArgs& A, long long i) {
 }
 
 // n / d for n * d < 2^32 with magic = ceil(2^32 / d) (the launcher keeps items * T below 2^16, heads * vectors below 2^24 with at most
-// 128 vectors a head); d = 1 has no 32-bit magic
+// 256 vectors a head); d = 1 has no 32-bit magic
 __device__ __forceinline__ unsigned quick_div(unsigned n, unsigned magic) { return magic ? __umulhi(n, magic) : n; }
 
 template <typename T, int V>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs A) {
-  extern __shared__ float2 table[];  // [T][D / 2]: identity behind the pairs, so that an interleaved vector may straddle the border
+  extern __shared__ float2 table[];  // [T][D / 2]; behind the pairs, where an interleaved vector may straddle the border, not used
   const long long t0 = (long long)blockIdx.x * A.T;
   const int nt = (int)min((long long)A.T, A.tokens - t0), half = A.D >> 1;
   for (int i = threadIdx.x; i < nt * half; i += 256) {
@@ -84,8 +84,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs A) {
         for (int k = 0; k < V; k += 2) {
           const float2 w = cs[(c * V + k) >> 1];
           const float lo = (float)a.v[k], hi = (float)a.v[k + 1];
-          o.v[k] = (T)(lo * w.x - hi * w.y);
-          o.v[k + 1] = (T)(hi * w.x + lo * w.y);
+          const bool turned = c * V + k < 2 * A.P;  // (behind the pairs: as they are, an Inf times the identity's zero would reach its neighbour)
+          o.v[k] = turned ? (T)(lo * w.x - hi * w.y) : a.v[k];
+          o.v[k + 1] = turned ? (T)(hi * w.x + lo * w.y) : a.v[k + 1];
         }
       }
       *reinterpret_cast<Vec<T, V>*>(dst + c * V) = o;
