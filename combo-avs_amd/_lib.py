@@ -224,20 +224,21 @@ _eager_graphs = weakref.WeakKeyDictionary()  # {autograd node recorded on the de
 
 
 def record(function, *args):
-    """function.apply(*args).  Autograd keeps ONE accumulation node per leaf, alive as long as any graph of the leaf, and that node remembers
-    the stream on which it was made.  If that is the default stream, a backward pass that is captured into a graph has to join it,
-    which ends the process when the capture does: so a call inside a capture refuses while a graph of one of its leaves that an eager call on the
-    default stream has recorded is alive."""
-    import torch
-    if torch.cuda.is_current_stream_capturing():
-        leaves = [t for t in args if torch.is_tensor(t) and t.requires_grad and t.is_leaf]
+    """function.apply(*args), args[0] a tensor of the device that the call runs on.  Autograd keeps ONE accumulation node per leaf, alive as long as
+    any graph of the leaf, and that node remembers the stream on which it was made.  If that is the default stream, a backward pass that is captured
+    into a graph has to join it, which ends the process when the capture does: so a call inside a capture refuses while a graph of one of its leaves
+    that an eager call on the default stream has recorded is alive."""
+    with device_of(args[0]) as stream:
+        capturing = _torch.cuda.is_current_stream_capturing()
+    if capturing:
+        leaves = [t for t in args if _torch.is_tensor(t) and t.requires_grad and t.is_leaf]
         if any(ref() is t for refs in list(_eager_graphs.values()) for ref in refs for t in leaves):
             raise RuntimeError("a graph is being captured while an eager autograd graph of the same leaf, recorded on the default stream, is "
                                "alive: drop its outputs (or detach them) before the capture, or record them on another stream")
         return function.apply(*args)
     out = function.apply(*args)
-    if out.grad_fn is not None and _raw_stream(_current_device()) == 0:
-        leaves = [weakref.ref(t) for t in args if torch.is_tensor(t) and t.requires_grad and t.is_leaf]
+    if stream == 0 and out.grad_fn is not None:
+        leaves = [weakref.ref(t) for t in args if _torch.is_tensor(t) and t.requires_grad and t.is_leaf]
         if leaves:
             _eager_graphs[out.grad_fn] = leaves
     return out
