@@ -5,6 +5,7 @@ this package falls back to PyTorch/CPU for an op that has a HIP kernel.
 """
 import ctypes
 import os
+import threading
 import weakref
 
 import torch as _torch
@@ -221,6 +222,7 @@ def recorded(*tensors):
 
 
 _eager_graphs = weakref.WeakKeyDictionary()  # {autograd node recorded on the default stream: its leaves (weak)}
+_eager_lock = threading.RLock()  # (a dictionary that another thread adds to cannot be gone through)
 
 
 def record(function, *args):
@@ -232,7 +234,9 @@ def record(function, *args):
         capturing = _torch.cuda.is_current_stream_capturing()
     if capturing:
         leaves = [t for t in args if _torch.is_tensor(t) and t.requires_grad and t.is_leaf]
-        if any(ref() is t for refs in list(_eager_graphs.values()) for ref in refs for t in leaves):
+        with _eager_lock:
+            alive = list(_eager_graphs.values())
+        if any(ref() is t for refs in alive for ref in refs for t in leaves):
             raise RuntimeError("a graph is being captured while an eager autograd graph of the same leaf, recorded on the default stream, is "
                                "alive: drop its outputs (or detach them) before the capture, or record them on another stream")
         return function.apply(*args)
@@ -240,7 +244,8 @@ def record(function, *args):
     if stream == 0 and out.grad_fn is not None:
         leaves = [weakref.ref(t) for t in args if _torch.is_tensor(t) and t.requires_grad and t.is_leaf]
         if leaves:
-            _eager_graphs[out.grad_fn] = leaves
+            with _eager_lock:
+                _eager_graphs[out.grad_fn] = leaves
     return out
 
 
