@@ -187,6 +187,7 @@ def check(code, what):
         raise HipError(f"{what} failed with hipError_t {code}")
 
 
+MAX_SIZE = 2 ** 31 - 1  # of a dimension that an entry point takes as an int (ctypes would pass the low 32 bits of a larger one)
 FLOAT_TYPES = {_torch.float32: 0, _torch.bfloat16: 1, _torch.float16: 2}  # dtype codes of the entry points that take several types
 
 # the current device and a device's current stream as plain integers: torch.cuda.current_stream() builds a Stream object, 4 us of a

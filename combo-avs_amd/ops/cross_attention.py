@@ -118,6 +118,8 @@ def cross_attention(q, k, v, kv_lengths=None, blocked=None, scale=None):
         raise ValueError(f"cross_attention: head dimension {D}: a multiple of 8, at most {MAX_HEAD_DIM}")
     if Hk < 1 or Hq % Hk:
         raise ValueError(f"cross_attention: {Hq} query heads on {Hk} key heads")
+    if max(*q.shape, *k.shape) > _lib.MAX_SIZE:
+        raise ValueError(f"cross_attention: sizes beyond 2^31: q {tuple(q.shape)}, k {tuple(k.shape)}")
     scale = float(D ** -0.5 if scale is None else scale)
     if not 1e-37 < scale < 2e38:
         raise ValueError(f"cross_attention: scale {scale}: positive and finite in fp32")

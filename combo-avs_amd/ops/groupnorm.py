@@ -155,6 +155,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation="none
         raise ValueError("group_norm_act: x must be channels-last (x.contiguous(memory_format=torch.channels_last), _3d for five dimensions)")
     if x.shape[2:].numel() > 1 << 30:
         raise ValueError("group_norm_act: more than 2^30 places in a map")
+    if x.shape[0] > _lib.MAX_SIZE:
+        raise ValueError(f"group_norm_act: {x.shape[0]} maps")
     if not x.is_cuda:
         raise RuntimeError("combo_avs_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
     how = (int(groups), float(eps), ACTIVATIONS[activation])

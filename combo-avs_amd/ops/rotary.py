@@ -80,6 +80,8 @@ def rotary_axes(x, positions, sections, base=10000.0, interleaved=False, shared_
         raise ValueError(f"rotary_axes: sections {sections}: 1 to {MAX_AXES} axes, not negative, at most half of the head dimension {D}")
     if D % 2 or D > MAX_HEAD_DIM:
         raise ValueError(f"rotary_axes: head dimension {D}: even, at most {MAX_HEAD_DIM}")
+    if max(x.shape) > _lib.MAX_SIZE:
+        raise ValueError(f"rotary_axes: sizes beyond 2^31: {tuple(x.shape)}")
     base = float(base)
     if not (base > 0 and math.isfinite(base)):
         raise ValueError(f"rotary_axes: base {base}")
