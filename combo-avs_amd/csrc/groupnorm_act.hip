@@ -46,30 +46,35 @@ __device__ __forceinline__ float polynomial(const float (&c)[N], float x) {
 }
 
 // The normal distribution function and its density d(z).  With a = |z| the tail is R(a) exp(-a^2 / 2), and R, which falls from 1 / 2 like
-// 1 / (a sqrt(2 pi)), is t (c0 + c1 t + ..) in t = 1 / (1 + s a): coefficients fitted here for the smallest relative error (weighted least squares over
-// a of 0 to 14.5), so the small side keeps its relative size.  16-bit maps: six terms, 4.6e-6 of the tail, 1 / 50 of half a step of fp16.  fp32 maps:
-// seven terms from a = 1 on (7e-8), below that 1 / 2 + z P(z^2) with P fitted likewise (7e-10), and the exponent in two pieces (its rounding alone would be
-// 1.4e-6 at z = -6): 7 u of either side, u = 2^-24, root mean square of GELU over a normal z 2.3e-8.
+// 1 / (a sqrt(2 pi)), is t (c0 + c1 t + ..) in t = 1 / (1 + s a) from a = 1 on, so the small side keeps its relative size; below that it is 1 / 2 + z P(z^2).
+// Coefficients fitted here for the smallest relative error (weighted least squares): 7e-8 and 7e-10.  FULL: the exponent in two pieces (its rounding
+// alone is 1.4e-6 of the value at z = -6) and a division, 7 u of either side, u = 2^-24; GELU over a normal z then has a root mean square error of 2.3e-8.
 template <bool FULL>
 __device__ __forceinline__ float normal_cdf(float z, float& density) {
+  constexpr float kTail[7] = {0.11167358f, 0.11232360f, 0.09767063f, 0.10959552f, -0.0027825537f, 0.13058622f, -0.059144225f};
+  constexpr float kCentre[6] = {0.39894229f, -0.06649036f, 0.009973324f, -0.0011863301f, 1.1348650e-4f, -7.6542565e-6f};
+  const float a = fminf(fabsf(z), 15.f);  // (exp(-15^2 / 2) is 0 in fp32; a stays finite)
+  const float h = a * a, x = -0.72134752f * h, u = fmaf(0.28f, a, 1.f);
+  float e = __builtin_amdgcn_exp2f(x), t;
   if constexpr (FULL) {
-    constexpr float kTail[7] = {0.11167358f, 0.11232360f, 0.09767063f, 0.10959552f, -0.0027825537f, 0.13058622f, -0.059144225f};
-    constexpr float kCentre[6] = {0.39894229f, -0.06649036f, 0.009973324f, -0.0011863301f, 1.1348650e-4f, -7.6542565e-6f};
-    const float a = fminf(fabsf(z), 15.f);  // (exp(-15^2 / 2) is 0 here, and 15^2 has a finite square's error below)
-    const float h = a * a, l = fmaf(a, a, -h), x = -0.72134752f * h;
-    const float rest = fmaf(h, -0.72134752f, -x) + fmaf(h, -9.6298149e-9f, -0.72134752f * l);
-    const float e0 = __builtin_amdgcn_exp2f(x), e = fmaf(0.69314718f * e0, rest, e0);
-    density = 0.39894228f * e;
-    if (a < 1.f) return fmaf(z, polynomial(kCentre, h), 0.5f);
-    const float t = 1.f / fmaf(0.28f, a, 1.f), tail = polynomial(kTail, t) * t * e;
-    return z < 0.f ? tail : 1.f - tail;
+    const float rest = fmaf(h, -0.72134752f, -x) + fmaf(h, -9.6298149e-9f, -0.72134752f * fmaf(a, a, -h));
+    e = fmaf(0.69314718f * e, rest, e);
+    t = 1.f / u;
   } else {
-    constexpr float kTail[6] = {0.12386069f, 0.12044134f, 0.13342951f, 0.015745264f, 0.18044983f, -0.073928952f};
-    const float t = quick_rcp(fmaf(0.31f, fabsf(z), 1.f)), e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
-    density = 0.39894228f * e;
-    const float tail = polynomial(kTail, t) * t * e;
-    return z < 0.f ? tail : 1.f - tail;
+    t = quick_rcp(u);
   }
+  density = 0.39894228f * e;
+  const float tail = polynomial(kTail, t) * t * e;
+  return a < 1.f ? fmaf(z, polynomial(kCentre, h), 0.5f) : z < 0.f ? tail : 1.f - tail;
+}
+
+// the same by one tail of six terms from a = 0 on, 4.6e-6 of it: 1 / 50 of half a step of fp16, for results that are rounded to 16 bits (forward, 40 x 256 x
+// 56 x 56: 49.7 us, 53.4 with the function above).  Slopes do not take it: their sums, dw and db, come back in fp32 and were
+// off by 3.5 u of their terms' sizes with it, 0.9 without.
+__device__ __forceinline__ float normal_cdf_16(float z) {
+  constexpr float kTail[6] = {0.12386069f, 0.12044134f, 0.13342951f, 0.015745264f, 0.18044983f, -0.073928952f};
+  const float t = quick_rcp(fmaf(0.31f, fabsf(z), 1.f)), tail = polynomial(kTail, t) * t * __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+  return z < 0.f ? tail : 1.f - tail;
 }
 
 // FULL: to the last digits of fp32; else to what a 16-bit result shows of them
@@ -78,6 +83,7 @@ __device__ __forceinline__ float act(float z) {
   if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;  // (a NaN stays one)
   if constexpr (ACT == ACT_SILU) return z * sigmoid<FULL>(z);
   if constexpr (ACT == ACT_GELU) {
+    if constexpr (!FULL) return z * normal_cdf_16(z);
     float d;
     return z * normal_cdf<FULL>(z, d);
   }
