@@ -64,8 +64,8 @@ __device__ __forceinline__ int length_of(const Args& A, int b) {
 
 // row-major LDS tile of 16-bit values.  The pitch is an odd number p of 16-byte chunks with p = 3, 7 or 9 (mod 16): 16 rows at the same chunk (a
 // b128 operand read) start in 16 different chunks of the 64 banks, and 4 rows x 2 neighbouring chunks (16 lanes of a transposed read) in 8, and
-// every address is one lane register plus an immediate.  Conflicts are left in a quarter of the LDS cycles (SQ_LDS_BANK_CONFLICT); a swizzle by
-// exclusive-or has none, but costs a register or an instruction per operand, of which the kernels are short: forward at 64 x 4096 x 4096 x 128
+// every address is one lane register plus an immediate.  Conflicts are left in a quarter of the LDS cycles (SQ_LDS_BANK_CONFLICT over
+// SQ_LDS_IDX_ACTIVE: 0.25 forward and dk / dv, 0.20 dq at 64 x 4096 x 4096 x 128); a swizzle by exclusive-or has none, but costs a register or an instruction per operand, of which the kernels are short: forward at 64 x 4096 x 4096 x 128
 // 1272 us with the swizzle, 997 with the pitch.
 template <int DP>
 struct Tile {
@@ -428,9 +428,10 @@ __global__ void __launch_bounds__(256, 2) cross_few_kernel(const Args A) {
 // tile t into probabilities, the matrix pipe forms the scores of tile t + 1 and adds the product of tile t - 1, all in one basic block, where the
 // compiler mixes them.  K and V have two LDS buffers each and one barrier a tile: K runs one tile ahead, V one behind.  The loads stand at the head
 // of a step (at its end: 720 us instead of 600).
-// Bound by the matrix and vector instructions together and, with both at work, by the power that lowers the clock to ~1.9 GHz: 64 x 4096 x 4096 x
-// 128 592 us = 930 TFLOP/s (one tile at a time: 997), 32 x 4099 x 15680 x 64 760 to 860 us (at 64 dimensions a score's exponential weighs twice as
-// much; without it 6 % less, without operand reads from LDS 18 %).  Tried without gain: 64 rows a wave (spills), more waves of smaller tiles, loads
+// Bound by the matrix and vector instructions together and, with both at work, by the power that lowers the clock to 1.9 to 2.1 of 2.4 GHz
+// (GRBM_GUI_ACTIVE over the kernel's time): 64 x 4096 x 4096 x 128 611 us = 900 TFLOP/s (one tile at a time: 997), 32 x 4099 x 15680 x 64 790 to 810 us
+// in a row of calls = 660 TFLOP/s and 850 to 890 after a pause or alone under a profiler (at 64 dimensions a score's exponential weighs twice as much;
+// without it 6 % less, without operand reads from LDS 18 %).  Tried without gain: 64 rows a wave (spills), more waves of smaller tiles, loads
 // two tiles ahead, no running maximum, chains of maxima and sums.
 template <int DP>
 struct Wide {

@@ -4,13 +4,13 @@
 // The backward pass recomputes z from x: nothing but mean and rstd is kept, and the activation costs no tensor of its own.
 //
 // Bound: HBM.  A thread owns V neighbouring channels (16 bytes where the channel count and the pointers allow it) and walks the tokens, so
-// per-channel constants stay in registers and all accesses are whole vectors.  Two shapes:
+// per-channel constants stay in registers and all accesses are vectors, of as many values as divide the channel count (one, if that is odd).  Two shapes:
 //   one launch   a workgroup owns one image and a few whole groups: it reads them for the statistics and again, out of the cache, for the
 //                result.  For maps whose slice per workgroup is small (the launch then costs more than the traffic).
 //   two launches partial statistics per (image, slice of tokens), then every workgroup of the second launch joins the partials of its own
 //                image - a few KB out of L2 - and writes its tokens.
 // 40 x 256 x 56 x 56 bf16 with SiLU (64 MB): forward 14 us for the statistics (4.6 TB/s) and 30 for the result (4.3), backward 32 for the sums (4.0)
-// and 38 for dx (5.0), where a copy reaches 5.15; 3 x 60 x 117 x 93 fp16 with GELU (3.9 MB): 7, 9, 9 and 9 us; one 256 x 7 x 7 frame: 6.5 us.
+// and 38 for dx (5.0), where a copy reaches 5.15; 3 x 60 x 117 x 93 fp16 with GELU (3.9 MB): 8, 9, 10 and 9 us; one 256 x 7 x 7 frame: 6.5 us.
 // Statistics: a thread sums x - K and (x - K)^2 with K its own first value of the channel, in fp32, and hands on (mean, M2); these are
 // joined as M2 = sum M2_i + sum n_i (mean_i - mean)^2.  K is one of the values, so the shift's cancellation is at most n_thread * 2^-24 of M2
 // whatever the offset of the map (a plain sum of squares loses everything once mean^2 > 2^24 var).  All sums have a fixed order.
@@ -584,7 +584,9 @@ size_t lds_floats(int range, int V) {
 }
 
 // slices of an image: the batch makes just under 1024 workgroups, four for each CU (40 images in 26 slices were 1040, and the CUs with five
-// of them finished last: 39 us against 31), with at least 16 tokens and 8 KiB in each
+// of them finished last: 39 us against 31), with at least 16 tokens and 8 KiB in each.  At most 256 an image, one a CU where there is but one: every
+// workgroup of the second launch joins all partials of its image, and with up to 1024 of them 1 x 256 x 112 x 112 bf16 takes 85 us forward and 155 in
+// training, with 256 27 and 53 (1 x 256 x 512 x 512, which has the work for it: 159 and 357 against 128 and 447)
 void choose_slices(NormArgs& A, int size) {
   long long by_bytes = ((long long)A.HW * A.C * size + 8191) / 8192;
   long long want = 1024 / A.B;
