@@ -65,8 +65,8 @@ __device__ __forceinline__ int length_of(const Args& A, int b) {
 // row-major LDS tile of 16-bit values.  The pitch is an odd number p of 16-byte chunks with p = 3, 7 or 9 (mod 16): 16 rows at the same chunk (a
 // b128 operand read) start in 16 different chunks of the 64 banks, and 4 rows x 2 neighbouring chunks (16 lanes of a transposed read) in 8, and
 // every address is one lane register plus an immediate.  Conflicts are left in a quarter of the LDS cycles (SQ_LDS_BANK_CONFLICT over
-// SQ_LDS_IDX_ACTIVE: 0.25 forward and dk / dv, 0.20 dq at 64 x 4096 x 4096 x 128); a swizzle by exclusive-or has none, but costs a register or an instruction per operand, of which the kernels are short: forward at 64 x 4096 x 4096 x 128
-// 1272 us with the swizzle, 997 with the pitch.
+// SQ_LDS_IDX_ACTIVE at 64 x 4096 x 4096 x 128: 0.25 forward and dk / dv, 0.20 dq); a swizzle by exclusive-or has none, but costs a register or an
+// instruction per operand, of which the kernels are short: forward at that size 1272 us with the swizzle, 997 with the pitch.
 template <int DP>
 struct Tile {
   static constexpr int PITCH = DP == 32 ? 56 : (DP == 64 ? 72 : 152);
